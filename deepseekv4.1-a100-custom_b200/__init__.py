@@ -8,4 +8,4 @@ hand-written CUDA through the C-ABI of csrc/libb200moe.so on the current torch s
 """
 from . import _lib  # noqa: F401
 
-__all__ = ["quant", "kernels", "moe_kernels", "fused", "fused2", "cukern", "w8", "ep", "moe", "synth"]
+__all__ = ["quant", "kernels", "moe_kernels", "fused", "fused2", "cukern", "w8", "ep", "moe", "dense", "synth"]

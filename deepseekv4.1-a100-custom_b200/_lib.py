@@ -14,6 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "csrc", "libb200moe.so")
 
 FMT_FP4_E8M0, FMT_FP4_BF16S, FMT_FP8_E8M0, FMT_FP8_F32B = 0, 1, 2, 3
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 SCORE_MODES = {"sqrtsoftplus": 0, "sigmoid": 1, "softmax": 2}
 
 c_p, c_i, c_ll, c_f, c_sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
@@ -92,6 +94,18 @@ _SIGNATURES = {
     "b200_group_pairs_workspace_bytes": (c_sz, [c_i]),
     "b200_group_pairs": (c_i, [c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p]),
     "b200_regroup_pairs": (c_i, [c_p, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p]),
+    "b200_add_rms_norm": (c_i, [c_p, c_ll, c_p, c_ll, c_p, c_i, c_i, c_ll, c_i, c_f, c_p, c_p, c_p, c_p, c_p]),
+    "b200_add_rms_norm_bwd_workspace_bytes": (c_sz, [c_ll, c_i]),
+    "b200_add_rms_norm_bwd": (c_i, [c_p, c_ll, c_p, c_ll, c_p, c_i, c_i, c_ll, c_i, c_f, c_p, c_p, c_p, c_p, c_p, c_sz, c_p]),
+    "b200_linear_act": (c_i, [c_p, c_ll, c_p, c_ll, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_ll, c_p, c_ll, c_p, c_ll, c_p]),
+    "b200_linear_act_bwd_workspace_bytes": (c_sz, [c_i, c_i]),
+    "b200_linear_act_bwd": (c_i, [c_p, c_ll, c_p, c_ll, c_i, c_i, c_i, c_i, c_p, c_ll, c_p, c_p, c_sz, c_p]),
+    "b200_gated_linear": (c_i, [c_p, c_ll, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_f, c_p, c_ll, c_p, c_ll, c_p]),
+    "b200_gated_linear_bwd": (c_i, [c_p, c_ll, c_p, c_ll, c_i, c_f, c_i, c_i, c_i, c_p, c_ll, c_p]),
+    "b200_dense_product": (c_i, [c_p, c_ll, c_i, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p, c_ll, c_p]),
+    "b200_align_rows": (c_i, [c_p, c_ll, c_p, c_ll, c_ll, c_i, c_p]),
+    "b200_linear_act_q8_workspace_bytes": (c_sz, [c_i, c_i, c_i]),
+    "b200_linear_act_q8": (c_i, [c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_ll, c_p, c_ll, c_p, c_sz, c_p]),
     "b200_scale_atoms_bytes": (c_sz, [c_i, c_i, c_i, c_i]),
     "b200_scale_atoms": (c_i, [c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_p]),
 }

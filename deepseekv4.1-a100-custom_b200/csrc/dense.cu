@@ -1,0 +1,270 @@
+// C entry points of the dense feed-forward operators: out = act(x W^T + bias) + residual and the gated product
+// act(x Wg^T) * (x Wu^T), with the element-wise halves of their backward passes.  The products are fgemm.cu's.
+#include <cuda_fp8.h>
+
+#include "b200_moe.h"
+#include "common.cuh"
+#include "dense.cuh"
+#include "fgemm.cuh"
+#include "ftypes.cuh"
+
+namespace b200 {
+
+// dz = gy * act'(z) and the column sums of dz.  8 warps of a block share DZ_ROWS rows of 32 * VEC columns; the sums of a block's rows go to
+// part[block row][N] in fp32 (from the unrounded dz), added in block order afterwards.  Bound by HBM: gy and z in, dz out.
+constexpr int DZ_ROWS = 64;
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const T* __restrict__ z, long long z_ld, int act, int M, int N,
+                                                      T* __restrict__ dz, long long dz_ld, float* __restrict__ part) {
+    __shared__ float red[8][32 * VEC];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = (blockIdx.x * 32 + lane) * VEC;
+    const int r_end = min(M, (int)(blockIdx.y + 1) * DZ_ROWS);
+    float sum[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+    if (c < N) {
+        for (int r = blockIdx.y * DZ_ROWS + warp; r < r_end; r += 8) {
+            float g[VEC];
+            load_vec<T, VEC>(gy + r * gy_ld + c, g);
+            if (z) {
+                float v[VEC];
+                load_vec<T, VEC>(z + r * z_ld + c, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) g[i] *= act_bwd(act, v[i]).y;
+            }
+            if (dz) store_vec<T, VEC>(dz + r * dz_ld + c, g);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum[i] += g[i];
+        }
+    }
+    if (!part) return;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) red[warp][i * 32 + lane] = sum[i];
+    __syncthreads();
+    for (int k = threadIdx.x; k < 32 * VEC; k += 256) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += red[w][k];
+        const int col = (blockIdx.x * 32 + (k & 31)) * VEC + (k >> 5);
+        if (col < N) part[(long long)blockIdx.y * N + col] = t;
+    }
+}
+
+// [dg | du] of the gated product from gy and the saved [g | u]: dg = gy u' act'(g') where the clamp let g through, du = gy act(g') where it
+// let u through (g', u': the clamped values).  Bound by HBM: 3 values in, 2 out per element of gy.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const T* __restrict__ gu, long long gu_ld, int act, float limit, long long M,
+                                                        int inter, T* __restrict__ dgu, long long dgu_ld) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int per_row = (inter + VEC - 1) / VEC;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long r = i / per_row;
+    if (r >= M) return;
+    const int c = (int)(i - r * per_row) * VEC;
+    float d[VEC], g[VEC], u[VEC];
+    load_vec<T, VEC>(gy + r * gy_ld + c, d);
+    load_vec<T, VEC>(gu + r * gu_ld + c, g);
+    load_vec<T, VEC>(gu + r * gu_ld + inter + c, u);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        bool pass_g = true, pass_u = true;
+        if (limit > 0.f) {  // clamped values were stored as 1.0625 limit (fgemm.cu); the others may have been rounded up to just above it
+            pass_g = !(g[k] > 1.03125f * limit);
+            pass_u = !(fabsf(u[k]) > 1.03125f * limit);
+            if (g[k] > limit) g[k] = limit;
+            if (fabsf(u[k]) > limit) u[k] = copysignf(limit, u[k]);
+        }
+        const float2 a = act_bwd(act, g[k]);
+        g[k] = pass_g ? d[k] * u[k] * a.y : 0.f;
+        u[k] = pass_u ? d[k] * a.x : 0.f;
+    }
+    store_vec<T, VEC>(dgu + r * dgu_ld + c, g);
+    store_vec<T, VEC>(dgu + r * dgu_ld + inter + c, u);
+}
+
+// rows of any width and address into rows that start on 16 bytes (dst_ld a multiple of 8): a tensor map needs that
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restrict__ src, long long src_ld, uint16_t* __restrict__ dst, long long dst_ld, long long rows,
+                                                         int cols) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int per_row = (cols + 7) / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
+    if (r >= rows) return;
+    const int c = (int)(i - r * per_row) * 8;
+    const uint16_t* s = src + r * src_ld + c;
+    uint32_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? s[k] : 0;  // the rest of the last 16 bytes: zeros
+    *reinterpret_cast<uint4*>(dst + r * dst_ld + c) = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+}
+
+// e4m3 codes with one E8M0 scale per 32 k (row r's scales in row r >> row_shift of sf) -> bf16, exactly: 4 significant bits times a power of two
+__global__ void __launch_bounds__(256) dequant_rows_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int sf_ld, int row_shift, long long rows, int K,
+                                                           __nv_bfloat16* __restrict__ out) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int per_row = K / 16;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
+    if (r >= rows) return;
+    const int c = (int)(i - r * per_row) * 16;
+    const uint4 raw = *reinterpret_cast<const uint4*>(q + r * K + c);
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w}, e = sf[(r >> row_shift) * sf_ld + (c >> 5)];
+    const float s = e ? u32_as_f32(e << 23) : 5.877471754111438e-39f;  // 2^(e - 127)
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(u[k >> 2] >> (8 * (k & 3))), __NV_E4M3))) * s;
+    store8<__nv_bfloat16>(out + r * K + c, *reinterpret_cast<const float(*)[8]>(&v[0]));
+    store8<__nv_bfloat16>(out + r * K + c + 8, *reinterpret_cast<const float(*)[8]>(&v[8]));
+}
+
+static bool ok16(const void* p, long long ld) { return !((uintptr_t)p & 15) && ld % 8 == 0; }
+
+template <typename T>
+static int act_bwd_run(const void* gy, long long gy_ld, const void* z, long long z_ld, int act, int M, int N, void* dz, long long dz_ld, float* part, cudaStream_t stream) {
+    const bool vec = N % 8 == 0 && ok16(gy, gy_ld) && (!z || ok16(z, z_ld)) && (!dz || ok16(dz, dz_ld));
+    const int w = vec ? 256 : 32;
+    const dim3 grid((N + w - 1) / w, (M + DZ_ROWS - 1) / DZ_ROWS);
+    return (int)launch_pdl(vec ? act_bwd_kernel<T, 8> : act_bwd_kernel<T, 1>, grid, dim3(256), 0, stream, (const T*)gy, gy_ld, (const T*)z, z_ld, act, M, N, (T*)dz, dz_ld,
+                           part);
+}
+
+template <typename T>
+static int gated_bwd_run(const void* gy, long long gy_ld, const void* gu, long long gu_ld, int act, float limit, int M, int inter, void* dgu, long long dgu_ld,
+                         cudaStream_t stream) {
+    const bool vec = inter % 8 == 0 && ok16(gy, gy_ld) && ok16(gu, gu_ld) && ok16(dgu, dgu_ld);
+    const long long threads = (long long)M * (vec ? inter / 8 : inter), blocks = (threads + 255) / 256;
+    if (blocks > 0x7FFFFFFFll) return ERR_TOO_LARGE;
+    return (int)launch_pdl(vec ? gated_bwd_kernel<T, 8> : gated_bwd_kernel<T, 1>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)gy, gy_ld, (const T*)gu, gu_ld, act,
+                           limit, (long long)M, inter, (T*)dgu, dgu_ld);
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+static int dense_check(int dtype, int act) {
+    if (dtype != F_BF16 && dtype != F_FP16) return ERR_UNSUPPORTED;
+    return act < ACT_NONE || act > ACT_GELU_TANH ? ERR_UNSUPPORTED : 0;
+}
+
+extern "C" int b200_linear_act(const void* x, long long x_ld, const void* w, long long w_ld, int dtype, int M, int N, int K, const void* bias, int act,
+                               const void* residual, long long r_ld, void* out, long long out_ld, void* z, long long z_ld, cudaStream_t stream) {
+    const int rc = dense_check(dtype, act);
+    if (rc) return rc;
+    if (M < 0 || N <= 0 || K <= 0) return ERR_BAD_SHAPE;
+    if (M == 0) return 0;
+    if (!x || !w || !out) return ERR_BAD_ARG;
+    if (out_ld < N || (residual && r_ld < N) || (z && z_ld < N)) return ERR_BAD_SHAPE;
+    FgArgs a{};
+    a.a = {x, x_ld, 0};
+    a.b = {w, w_ld, 0};
+    a.M = M; a.N = N; a.K = K; a.is_f16 = dtype == F_FP16;
+    a.act = act; a.bias = bias; a.res = residual; a.res_ld = r_ld; a.out = out; a.out_ld = out_ld; a.z_out = z; a.z_ld = z_ld;
+    return fg_launch(a, stream);
+}
+
+extern "C" int b200_gated_linear(const void* x, long long x_ld, const void* w13, long long w_ld, int dtype, int M, int inter, int K, int act, float limit, void* out,
+                                 long long out_ld, void* gu, long long gu_ld, cudaStream_t stream) {
+    const int rc = dense_check(dtype, act);
+    if (rc) return rc;
+    if (M < 0 || inter <= 0 || inter > (1 << 29) || K <= 0 || !(limit >= 0.f)) return ERR_BAD_SHAPE;
+    if (M == 0) return 0;
+    if (!x || !w13 || !out) return ERR_BAD_ARG;
+    if (out_ld < inter || (gu && gu_ld < 2 * inter)) return ERR_BAD_SHAPE;
+    FgArgs a{};
+    a.a = {x, x_ld, 0};
+    a.b = {w13, w_ld, 0};
+    a.M = M; a.N = 2 * inter; a.K = K; a.is_f16 = dtype == F_FP16;
+    a.dual = 1; a.inter = inter; a.act = act; a.limit = limit; a.out = out; a.out_ld = out_ld; a.z_out = gu; a.z_ld = gu_ld;
+    return fg_launch(a, stream);
+}
+
+extern "C" int b200_dense_product(const void* a_base, long long a_ld, int a_mn, const void* b_base, long long b_ld, int b_mn, int dtype, int M, int N, int K, void* out,
+                                  long long out_ld, cudaStream_t stream) {
+    const int rc = dense_check(dtype, 0);
+    if (rc) return rc;
+    if (M < 0 || N < 0 || K <= 0 || out_ld < N) return ERR_BAD_SHAPE;
+    if (M == 0 || N == 0) return 0;
+    if (!a_base || !b_base || !out) return ERR_BAD_ARG;
+    FgArgs a{};
+    a.a = {a_base, a_ld, a_mn != 0};
+    a.b = {b_base, b_ld, b_mn != 0};
+    a.M = M; a.N = N; a.K = K; a.is_f16 = dtype == F_FP16;
+    a.out = out; a.out_ld = out_ld;
+    return fg_launch(a, stream);
+}
+
+extern "C" size_t b200_linear_act_bwd_workspace_bytes(int M, int N) {
+    if (M <= 0 || N <= 0) return 0;
+    return (size_t)((M + DZ_ROWS - 1) / DZ_ROWS) * (size_t)N * sizeof(float);
+}
+
+extern "C" int b200_linear_act_bwd(const void* gy, long long gy_ld, const void* z, long long z_ld, int act, int dtype, int M, int N, void* dz, long long dz_ld, void* dbias,
+                                   void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    const int rc = dense_check(dtype, act);
+    if (rc) return rc;
+    if (M < 0 || N <= 0) return ERR_BAD_SHAPE;
+    if (act != ACT_NONE && M > 0 && !z) return ERR_BAD_ARG;
+    if (M == 0) return dbias ? (int)cudaMemsetAsync(dbias, 0, (size_t)N * 2, stream) : 0;
+    if (!gy || (!dz && !dbias)) return ERR_BAD_ARG;
+    if (gy_ld < N || (z && z_ld < N) || (dz && dz_ld < N)) return ERR_BAD_SHAPE;
+    if ((M + DZ_ROWS - 1) / DZ_ROWS > 65535) return ERR_TOO_LARGE;
+    if (dbias && (!workspace || workspace_bytes < b200_linear_act_bwd_workspace_bytes(M, N))) return ERR_WORKSPACE;
+    float* part = dbias ? (float*)workspace : nullptr;
+    if (act == ACT_NONE) z = nullptr;
+    const int e = dtype == F_BF16 ? act_bwd_run<__nv_bfloat16>(gy, gy_ld, z, z_ld, act, M, N, dz, dz_ld, part, stream)
+                                  : act_bwd_run<__half>(gy, gy_ld, z, z_ld, act, M, N, dz, dz_ld, part, stream);
+    if (e || !dbias) return e;
+    return column_sum(part, (M + DZ_ROWS - 1) / DZ_ROWS, N, dtype, dbias, stream);
+}
+
+extern "C" int b200_gated_linear_bwd(const void* gy, long long gy_ld, const void* gu, long long gu_ld, int act, float limit, int dtype, int M, int inter, void* dgu,
+                                     long long dgu_ld, cudaStream_t stream) {
+    const int rc = dense_check(dtype, act);
+    if (rc) return rc;
+    if (M < 0 || inter <= 0 || inter > (1 << 29) || !(limit >= 0.f)) return ERR_BAD_SHAPE;
+    if (M == 0) return 0;
+    if (!gy || !gu || !dgu) return ERR_BAD_ARG;
+    if (gy_ld < inter || gu_ld < 2 * inter || dgu_ld < 2 * inter) return ERR_BAD_SHAPE;
+    return dtype == F_BF16 ? gated_bwd_run<__nv_bfloat16>(gy, gy_ld, gu, gu_ld, act, limit, M, inter, dgu, dgu_ld, stream)
+                           : gated_bwd_run<__half>(gy, gy_ld, gu, gu_ld, act, limit, M, inter, dgu, dgu_ld, stream);
+}
+
+extern "C" int b200_align_rows(const void* src, long long src_ld, void* dst, long long dst_ld, long long rows, int cols, cudaStream_t stream) {
+    if (rows < 0 || cols <= 0 || src_ld < 0 || dst_ld < cols) return ERR_BAD_SHAPE;
+    if (rows == 0) return 0;
+    if (!src || !dst) return ERR_BAD_ARG;
+    if (((uintptr_t)src & 1) || !ok16(dst, dst_ld)) return ERR_BAD_ALIGN;
+    const long long blocks = (rows * ((cols + 7) / 8) + 255) / 256;
+    if (blocks > 0x7FFFFFFFll) return ERR_TOO_LARGE;
+    return (int)launch_pdl(align_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (const uint16_t*)src, src_ld, (uint16_t*)dst, dst_ld, rows, cols);
+}
+
+extern "C" size_t b200_linear_act_q8_workspace_bytes(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return ((size_t)M + N) * (size_t)K * 2;
+}
+
+extern "C" int b200_linear_act_q8(const void* x8, const void* xsf, const void* w8, const void* s8, int s_cols, int M, int N, int K, const void* bias, int act,
+                                  const void* residual, long long r_ld, void* out, long long out_ld, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    const int rc = dense_check(F_BF16, act);
+    if (rc) return rc;
+    if (M < 0 || N <= 0 || K <= 0 || K % 128 || s_cols < K / 32) return ERR_BAD_SHAPE;
+    if (M == 0) return 0;
+    if (!x8 || !xsf || !w8 || !s8 || !out) return ERR_BAD_ARG;
+    if (out_ld < N || (residual && r_ld < N)) return ERR_BAD_SHAPE;
+    if (((uintptr_t)x8 & 15) || ((uintptr_t)w8 & 15)) return ERR_BAD_ALIGN;
+    if (!workspace || workspace_bytes < b200_linear_act_q8_workspace_bytes(M, N, K)) return ERR_WORKSPACE;
+    if ((uintptr_t)workspace & 15) return ERR_BAD_ALIGN;
+    __nv_bfloat16 *xb = (__nv_bfloat16*)workspace, *wb = xb + (size_t)M * K;
+    const long long bx = ((long long)M * (K / 16) + 255) / 256, bw = ((long long)N * (K / 16) + 255) / 256;
+    if (bx > 0x7FFFFFFFll || bw > 0x7FFFFFFFll) return ERR_TOO_LARGE;
+    cudaError_t e = launch_pdl(dequant_rows_kernel, dim3((unsigned)bx), dim3(256), 0, stream, (const uint8_t*)x8, (const uint8_t*)xsf, K / 32, 0, (long long)M, K, xb);
+    if (e == cudaSuccess) e = launch_pdl(dequant_rows_kernel, dim3((unsigned)bw), dim3(256), 0, stream, (const uint8_t*)w8, (const uint8_t*)s8, s_cols, 5, (long long)N, K, wb);
+    if (e != cudaSuccess) return (int)e;
+    return b200_linear_act(xb, K, wb, K, F_BF16, M, N, K, bias, act, residual, r_ld, out, out_ld, nullptr, 0, stream);
+}

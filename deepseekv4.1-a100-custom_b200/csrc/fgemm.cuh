@@ -1,0 +1,39 @@
+// Internal interface of the 16-bit tensor-core GEMM (fgemm.cu): bf16 x bf16 or fp16 x fp16 with fp32 accumulation.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200 {
+
+// out[m, n] = epilogue( sum_k A[m, k] * B[n, k] ).  Either operand may lie with the contraction contiguous ("K-major": element (i, k) at
+// base[i * ld + k]) or with its rows contiguous ("MN-major": element (i, k) at base[k * ld + i]); the tensor cores read both, so the
+// products of the backward pass need no transposed copy.  Bases 16-byte aligned, ld a multiple of 8 elements.
+struct FgOperand {
+    const void* base;
+    long long ld;
+    int mn_major;
+};
+
+struct FgArgs {
+    FgOperand a, b;
+    int M, N, K;             // N counts the rows of B (2 * inter with dual)
+    int is_f16;              // 0: bf16, 1: fp16 (operands, bias, residual and outputs)
+    // epilogue: z = acc + bias;  out = act(z) + res;  z is stored too when z_out is given.
+    // dual: B's rows are [gate | up], columns j and inter + j meet in one thread: out = act(min(g, limit)) * clamp(u, +-limit) (limit 0: no clamp);
+    // z_out receives [g | u]
+    int dual, inter;
+    int act;
+    float limit;
+    const void* bias;
+    const void* res;
+    long long res_ld;
+    void* out;
+    long long out_ld;
+    void* z_out;
+    long long z_ld;
+};
+
+int fg_launch(const FgArgs& a, cudaStream_t stream);
+int fg_device_error(int* out);  // device error word (a wait that ran out of time), read and cleared
+
+}  // namespace b200

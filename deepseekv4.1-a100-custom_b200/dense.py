@@ -1,0 +1,365 @@
+"""Dense feed-forward operators around the MoE path: the residual stream with its norm (`add_rms_norm`, `add_rms_norm_quant`), a projection with
+bias, activation and residual in its epilogue (`linear_act`, `linear_act_q8`), the gated projection (`gated_linear`), and the block they form
+(`DenseFFN`).  All are kernels of the library (include/b200_moe.h, "dense feed-forward operators") launched on the current stream of the
+tensors' device; nothing synchronises.  Scratch and outputs come from torch's allocator per call, so calls on several streams, and captured
+CUDA graphs, share no memory.
+
+`add_rms_norm`, `linear_act` and `gated_linear` are differentiable (once); the FP8 forms are for serving and refuse inputs that require a
+gradient.  A captured backward pass needs what torch asks of any: capture it on the stream that ran the warm-up, and drop eager graphs of the
+same leaves first."""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+_PAIR = (torch.bfloat16, torch.float16)
+
+
+# ------------------------------------------------------------------ marshalling
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., D] as rows [R, D] with a unit inner stride and rows that do not overlap (a copy only where the strides do not allow a view)."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _pitch(n: int) -> int:
+    return (n + 7) // 8 * 8
+
+
+def _tma_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """Rows as the tensor-core kernels fetch them: 16-byte aligned base, stride a multiple of 8 elements; other rows are copied once."""
+    t = _rows(t)
+    r, d = t.shape
+    if t.data_ptr() % 16 == 0 and (r == 1 or t.stride(0) % 8 == 0):
+        return t, t.stride(0) if r > 1 else _pitch(d)
+    ld = _pitch(d)
+    out = torch.empty(r, ld, device=t.device, dtype=t.dtype)
+    L.check(L.lib().b200_align_rows(L.ptr(t), _ld(t), L.ptr(out), ld, r, d, L.stream_of(t.device)), "b200_align_rows")
+    return out[:, :d], ld
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K) -> torch.Tensor:
+    out = torch.empty(M, N, device=a.device, dtype=a.dtype)
+    L.check(L.lib().b200_dense_product(L.ptr(a), a_ld, a_mn, L.ptr(b), b_ld, b_mn, L.DTYPES[a.dtype], M, N, K, L.ptr(out), N, L.stream_of(a.device)), "b200_dense_product")
+    return out
+
+
+def _empty_scratch(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+# ------------------------------------------------------------------ residual addition + rms norm
+def _norm_args(x, residual, weight, eps):
+    dev = L.require_cuda(x, residual, weight)
+    D = x.shape[-1]
+    assert x.dtype in L.DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}"
+    assert 1 <= D <= 16384, f"width {D} is outside 1..16384"
+    assert residual is None or (residual.dtype == x.dtype and residual.shape == x.shape), "residual must have the type and shape of x"
+    assert weight is None or (weight.shape == (D,) and weight.dtype in (x.dtype, torch.float32)), "weight must be [D], in x's type or float32"
+    assert eps >= 0.0, "eps must not be negative"
+    return dev, D
+
+
+def _norm_forward(x, residual, weight, eps, y, s, q8, sf):
+    """x, residual: 2-D rows; weight contiguous."""
+    L.check(L.lib().b200_add_rms_norm(L.ptr(x), _ld(x), L.ptr(residual), _ld(residual) if residual is not None else 0, L.ptr(weight),
+                                      int(weight is not None and weight.dtype == torch.float32), L.DTYPES[x.dtype], x.shape[0], x.shape[1], float(eps), L.ptr(y), L.ptr(s),
+                                      L.ptr(q8), L.ptr(sf), L.stream_of(x.device)), "b200_add_rms_norm")
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        x2, r2 = _rows(x), _rows(residual) if residual is not None else None
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        s = torch.empty_like(y) if residual is not None else None
+        wc = weight.contiguous() if weight is not None else None
+        with torch.cuda.device(x.device):
+            _norm_forward(x2, r2, wc, eps, y, s, None, None)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x2, r2, wc)
+        ctx.eps, ctx.shape = eps, x.shape
+        return (y, s) if residual is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gs=None):
+        x, r, w = ctx.saved_tensors
+        need_x, need_r, need_w, _ = ctx.needs_input_grad
+        if gy is None:  # the normed output was not used
+            dw = torch.zeros_like(w) if need_w else None
+            return gs if need_x else None, gs if need_r else None, dw, None
+        dev = x.device
+        gy = gy.contiguous()
+        gs = gs.contiguous() if gs is not None else None
+        rows, D = x.shape
+        ds = torch.empty(ctx.shape, device=dev, dtype=x.dtype)
+        dw = torch.empty_like(w) if need_w else None
+        with torch.cuda.device(dev):
+            lib = L.lib()
+            nb = lib.b200_add_rms_norm_bwd_workspace_bytes(rows, D) if need_w else 0
+            ws = _empty_scratch(nb, dev) if nb else None
+            L.check(lib.b200_add_rms_norm_bwd(L.ptr(x), _ld(x), L.ptr(r), _ld(r) if r is not None else 0, L.ptr(w), int(w is not None and w.dtype == torch.float32),
+                                              L.DTYPES[x.dtype], rows, D, float(ctx.eps), L.ptr(gy), L.ptr(gs), L.ptr(ds), L.ptr(dw), L.ptr(ws), nb, L.stream_of(dev)),
+                    "b200_add_rms_norm_bwd")
+        return ds if need_x else None, ds if need_r else None, dw, None
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """x, residual [..., D] bf16 | fp16 | fp32 -> (y, s): s = x + residual (x itself without a residual), y = s / sqrt(mean(s^2) + eps) * weight.
+    The norm is taken of the unrounded fp32 sum.  weight [D] in x's type or fp32, or None for ones.  Differentiable."""
+    _norm_args(x, residual, weight, eps)
+    if _wants_grad(x, residual, weight):
+        out = _AddRmsNorm.apply(x, residual, weight, float(eps))
+        return out if residual is not None else (out, x)
+    x2, r2 = _rows(x), _rows(residual) if residual is not None else None
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    s = torch.empty_like(y) if residual is not None else None
+    with torch.cuda.device(x.device):
+        _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, eps, y, s, None, None)
+    return y, (s if residual is not None else x)
+
+
+def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6, want_y: bool = False):
+    """The same norm with y in 8 bits -> (q8, sf, s[, y]): q8 uint8 e4m3 codes [rows, D], sf uint8 E8M0 [rows, D/32], rows = all leading
+    dimensions together (what `cukern.mx_grouped` and `linear_act_q8` take); q8 * 2^(sf - 127) is y quantised per 32 from its fp32 value.  want_y:
+    y in x's type too.  D % 32 == 0.  No gradient."""
+    dev, D = _norm_args(x, residual, weight, eps)
+    assert D % 32 == 0, f"width {D} is not a multiple of 32"
+    assert not _wants_grad(x, residual, weight), "add_rms_norm_quant has no gradient: use add_rms_norm, or detach its inputs"
+    x2, r2 = _rows(x), _rows(residual) if residual is not None else None
+    rows = x2.shape[0]
+    q8 = torch.empty(rows, D, device=dev, dtype=torch.uint8)
+    sf = torch.empty(rows, D // 32, device=dev, dtype=torch.uint8)
+    s = torch.empty(x.shape, device=dev, dtype=x.dtype) if residual is not None else None
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype) if want_y else None
+    with torch.cuda.device(dev):
+        _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, eps, y, s, q8, sf)
+    s = s if residual is not None else x
+    return (q8, sf, s, y) if want_y else (q8, sf, s)
+
+
+# ------------------------------------------------------------------ projection with bias, activation, residual
+def _linear_forward(x, x_ld, w, w_ld, bias, act, residual, out, z, z_ld):
+    M, K = x.shape
+    N = w.shape[0]
+    r_ld = _ld(residual) if residual is not None else 0
+    L.check(L.lib().b200_linear_act(L.ptr(x), x_ld, L.ptr(w), w_ld, L.DTYPES[x.dtype], M, N, K, L.ptr(bias), act, L.ptr(residual), r_ld, L.ptr(out), N, L.ptr(z), z_ld,
+                                    L.stream_of(x.device)), "b200_linear_act")
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, act, residual):
+        M_shape, N = x.shape[:-1], w.shape[0]
+        with torch.cuda.device(x.device):
+            x2, x_ld = _tma_rows(x)
+            w2, w_ld = _tma_rows(w)
+            r2 = _rows(residual) if residual is not None else None
+            b = bias.contiguous() if bias is not None else None
+            out = torch.empty(*M_shape, N, device=x.device, dtype=x.dtype)
+            z_ld = _pitch(N)
+            z = torch.empty(x2.shape[0], z_ld, device=x.device, dtype=x.dtype) if act else None
+            _linear_forward(x2, x_ld, w2, w_ld, b, act, r2, out, z, z_ld)
+        ctx.save_for_backward(x2, w2, z)
+        ctx.x_ld, ctx.w_ld, ctx.act, ctx.x_shape = x_ld, w_ld, act, x.shape
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, w, z = ctx.saved_tensors
+        need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
+        (M, K), N, dev, lib = x.shape, w.shape[0], x.device, L.lib()
+        g2 = _rows(gy)
+        dx = dw = db = None
+        with torch.cuda.device(dev):
+            if need_b:
+                db = torch.empty(N, device=dev, dtype=x.dtype)
+            dz, dz_ld = g2, _ld(g2)
+            if (need_x or need_w) and (ctx.act or N % 8):
+                dz_ld = _pitch(N)
+                dz = torch.empty(M, dz_ld, device=dev, dtype=x.dtype)
+            if dz is not g2 or need_b:
+                nb = lib.b200_linear_act_bwd_workspace_bytes(M, N) if need_b else 0
+                ws = _empty_scratch(nb, dev) if nb else None
+                L.check(lib.b200_linear_act_bwd(L.ptr(g2), _ld(g2), L.ptr(z), _pitch(N) if z is not None else 0, ctx.act, L.DTYPES[x.dtype], M, N,
+                                                L.ptr(dz) if dz is not g2 else None, dz_ld, L.ptr(db), L.ptr(ws), nb, L.stream_of(dev)), "b200_linear_act_bwd")
+            if (need_x or need_w) and dz is g2:
+                dz, dz_ld = _tma_rows(g2)
+            if need_x:
+                dx = _product(dz, dz_ld, 0, w, ctx.w_ld, 1, M, K, N).view(ctx.x_shape)
+            if need_w:
+                dw = _product(dz, dz_ld, 1, x, ctx.x_ld, 1, N, K, M) if M else torch.zeros(N, K, device=dev, dtype=x.dtype)
+        return dx, dw, db, None, gy if need_r else None
+
+
+def _act_code(act) -> int:
+    assert act in L.ACTIVATIONS, f"act must be one of {sorted(a for a in L.ACTIVATIONS if a)} or None, got {act!r}"
+    return L.ACTIVATIONS[act]
+
+
+def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x w^T + bias) + residual: x [..., K], w [N, K], bias [N], residual [..., N], all bf16 or all fp16; act None, "relu", "silu", "gelu"
+    (z Phi(z)) or "gelu_tanh".  fp32 accumulation, one rounding at the end.  Any K, N and number of rows; rows of x or w that do not start on
+    16 bytes (a K that is no multiple of 8, an odd slice) are copied first.  Differentiable in x, w, bias and residual."""
+    L.require_cuda(x, w, bias, residual)
+    code = _act_code(act)
+    assert x.dtype in _PAIR and w.dtype == x.dtype and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
+    N, K = w.shape
+    assert x.dim() >= 1 and x.shape[-1] == K and K >= 1 and N >= 1, f"x {tuple(x.shape)} does not fit w {tuple(w.shape)}"
+    assert bias is None or (bias.shape == (N,) and bias.dtype == x.dtype), "bias must be [N] in x's type"
+    assert residual is None or (residual.shape == (*x.shape[:-1], N) and residual.dtype == x.dtype), "residual must have the type and shape of the result"
+    if _wants_grad(x, w, bias, residual):
+        return _LinearAct.apply(x, w, bias, code, residual)
+    out = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
+    with torch.cuda.device(x.device):
+        x2, x_ld = _tma_rows(x)
+        w2, w_ld = _tma_rows(w)
+        _linear_forward(x2, x_ld, w2, w_ld, bias.contiguous() if bias is not None else None, code, _rows(residual) if residual is not None else None, out, None, 0)
+    return out
+
+
+def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None,
+                  residual: torch.Tensor | None = None) -> torch.Tensor:
+    """The projection on FP8 operands: x8 uint8 e4m3 [rows, K] + xsf uint8 E8M0 [rows, K/32] (`add_rms_norm_quant`, `cukern.mx_quantize_rows`), w8
+    uint8 e4m3 [N, K] in natural k order (`w8.unpermute_k` of a W8's bytes) + s8 uint8 E8M0 [ceil(N/32), K/32].  bias [N], residual [rows, N] and
+    the result bf16; products and sums in fp32.  K % 128 == 0.  No gradient."""
+    dev = L.require_cuda(x8, xsf, w8, s8, bias, residual)
+    code = _act_code(act)
+    assert all(t.dtype == torch.uint8 and t.dim() == 2 for t in (x8, xsf, w8, s8)), "x8, xsf, w8 and s8 are uint8 matrices"
+    (M, K), N = x8.shape, w8.shape[0]
+    assert K % 128 == 0 and K > 0 and w8.shape[1] == K and N >= 1, f"x8 {tuple(x8.shape)} / w8 {tuple(w8.shape)}: the widths must be equal and a multiple of 128"
+    assert xsf.shape == (M, K // 32) and s8.shape[0] == (N + 31) // 32 and s8.shape[1] >= K // 32, "one scale per 32 k: xsf [rows, K/32], s8 [ceil(N/32), K/32]"
+    assert bias is None or (bias.shape == (N,) and bias.dtype == torch.bfloat16), "bias must be bfloat16 [N]"
+    assert residual is None or (residual.shape == (M, N) and residual.dtype == torch.bfloat16), "residual must be bfloat16 [rows, N]"
+    assert not _wants_grad(bias, residual), "linear_act_q8 has no gradient"
+    x8, xsf, w8, s8 = (t.contiguous() for t in (x8, xsf, w8, s8))
+    r2 = _rows(residual) if residual is not None else None
+    out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
+    with torch.cuda.device(dev):
+        lib = L.lib()
+        nb = lib.b200_linear_act_q8_workspace_bytes(M, N, K)
+        ws = _empty_scratch(nb, dev) if nb else None
+        L.check(lib.b200_linear_act_q8(L.ptr(x8), L.ptr(xsf), L.ptr(w8), L.ptr(s8), s8.shape[1], M, N, K, L.ptr(bias.contiguous() if bias is not None else None), code,
+                                       L.ptr(r2), _ld(r2) if r2 is not None else 0, L.ptr(out), N, L.ptr(ws), nb, L.stream_of(dev)), "b200_linear_act_q8")
+    return out
+
+
+# ------------------------------------------------------------------ gated projection
+def _gated_forward(x, x_ld, w, w_ld, act, limit, out, gu, gu_ld):
+    M, K = x.shape
+    inter = w.shape[0] // 2
+    L.check(L.lib().b200_gated_linear(L.ptr(x), x_ld, L.ptr(w), w_ld, L.DTYPES[x.dtype], M, inter, K, act, float(limit), L.ptr(out), inter, L.ptr(gu), gu_ld,
+                                      L.stream_of(x.device)), "b200_gated_linear")
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, act, limit):
+        inter = w13.shape[0] // 2
+        with torch.cuda.device(x.device):
+            x2, x_ld = _tma_rows(x)
+            w2, w_ld = _tma_rows(w13)
+            out = torch.empty(*x.shape[:-1], inter, device=x.device, dtype=x.dtype)
+            gu_ld = _pitch(2 * inter)
+            gu = torch.empty(x2.shape[0], gu_ld, device=x.device, dtype=x.dtype)
+            _gated_forward(x2, x_ld, w2, w_ld, act, limit, out, gu, gu_ld)
+        ctx.save_for_backward(x2, w2, gu)
+        ctx.x_ld, ctx.w_ld, ctx.act, ctx.limit, ctx.x_shape = x_ld, w_ld, act, limit, x.shape
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, w, gu = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        (M, K), n2, dev = x.shape, w.shape[0], x.device
+        g2 = _rows(gy)
+        gu_ld = _pitch(n2)
+        dx = dw = None
+        with torch.cuda.device(dev):
+            dgu = torch.empty(M, gu_ld, device=dev, dtype=x.dtype)
+            L.check(L.lib().b200_gated_linear_bwd(L.ptr(g2), _ld(g2), L.ptr(gu), gu_ld, ctx.act, float(ctx.limit), L.DTYPES[x.dtype], M, n2 // 2, L.ptr(dgu), gu_ld,
+                                                  L.stream_of(dev)), "b200_gated_linear_bwd")
+            if need_x:
+                dx = _product(dgu, gu_ld, 0, w, ctx.w_ld, 1, M, K, n2).view(ctx.x_shape)
+            if need_w:
+                dw = _product(dgu, gu_ld, 1, x, ctx.x_ld, 1, n2, K, M) if M else torch.zeros(n2, K, device=dev, dtype=x.dtype)
+        return dx, dw, None, None
+
+
+def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", limit: float = 0.0) -> torch.Tensor:
+    """act(min(g, limit)) * min(max(u, -limit), limit) with [g | u] = x w13^T, both projections and the product in one kernel: x [..., K], w13
+    [2 * inter, K] (gate rows, then up rows: the layout of the expert weights), both bf16 or both fp16 -> [..., inter].  limit 0: no clamps.
+    Differentiable in x and w13; a call that needs a gradient also keeps g and u (2 * inter values per row)."""
+    L.require_cuda(x, w13)
+    code = _act_code(act)
+    assert x.dtype in _PAIR and w13.dtype == x.dtype and w13.dim() == 2, "x and w13 must be both bfloat16 or both float16, w13 [2 * inter, K]"
+    n2, K = w13.shape
+    assert n2 >= 2 and n2 % 2 == 0 and K >= 1 and x.dim() >= 1 and x.shape[-1] == K, f"x {tuple(x.shape)} does not fit w13 {tuple(w13.shape)}"
+    assert limit >= 0.0, "limit must not be negative"
+    if _wants_grad(x, w13):
+        return _GatedLinear.apply(x, w13, code, float(limit))
+    out = torch.empty(*x.shape[:-1], n2 // 2, device=x.device, dtype=x.dtype)
+    with torch.cuda.device(x.device):
+        x2, x_ld = _tma_rows(x)
+        w2, w_ld = _tma_rows(w13)
+        _gated_forward(x2, x_ld, w2, w_ld, code, limit, out, None, 0)
+    return out
+
+
+# ------------------------------------------------------------------ the block
+class DenseFFN:
+    """A non-expert feed-forward block on the residual stream: s = x + residual; h = gated_linear(norm(s), w13); returns h w2^T + s, the stream
+    behind the block.
+
+    w13 [2 * inter, D] and w2 [D, inter]: bf16 or fp16 tensors (trainable: every step is differentiable), or `W8` containers with E8M0 scales (D and
+    inter multiples of 128, serving only): the normed rows and the gated product then stay in 8 bits between the steps.  A natural-k-order copy of
+    the W8 bytes is made once here, as MoELayer does for the shared expert."""
+
+    def __init__(self, norm_weight: torch.Tensor | None, w13, w2, *, eps: float = 1e-6, act: str = "silu", limit: float = 0.0):
+        from .w8 import W8, unpermute_k
+        self.norm_weight, self.eps, self.act, self.limit = norm_weight, eps, act, limit
+        self.w13, self.w2 = w13, w2
+        self.inter, self.dim = w13.shape[0] // 2, w13.shape[1]
+        assert tuple(w2.shape) == (self.dim, self.inter) and w13.shape[0] == 2 * self.inter, f"w13 {tuple(w13.shape)} does not fit w2 {tuple(w2.shape)}"
+        _act_code(act)
+        self._nat = None
+        if isinstance(w13, W8) or isinstance(w2, W8):
+            assert isinstance(w13, W8) and isinstance(w2, W8) and w13.s8.dtype == torch.uint8 and w2.s8.dtype == torch.uint8, "w13 and w2: two W8 with E8M0 scales"
+            assert self.dim % 128 == 0 and self.inter % 128 == 0 and act == "silu", "the FP8 block needs widths that are multiples of 128 and act 'silu'"
+            self._nat = (unpermute_k(w13.w8), unpermute_k(w2.w8))
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """x, residual [..., D] -> [..., D]."""
+        if self._nat is None:
+            y, s = add_rms_norm(x, residual, self.norm_weight, self.eps)
+            return linear_act(gated_linear(y, self.w13, self.act, self.limit), self.w2, residual=s)
+        from . import cukern
+        assert x.dtype == torch.bfloat16, "the FP8 block takes bfloat16 activations"
+        q8, sf, s = add_rms_norm_quant(x, residual, self.norm_weight, self.eps)
+        T = q8.shape[0]
+        if T == 0:
+            return s
+        tpw = 128 if T > 64 else 32
+        rows = 128
+        while rows > 32 and (T + tpw - 1) // tpw * (self.inter // rows) < 148:
+            rows //= 2
+        h8, hsf = cukern.mx_grouped(self._nat[0], self.w13.s8, q8, sf, None, None, None, None, None, T, epilogue="swiglu_q8", limit=self.limit, tokens_per_work=tpw,
+                                    rows_per_tile=rows)
+        return linear_act_q8(h8, hsf, self._nat[1], self.w2.s8, residual=s.reshape(T, self.dim)).view(x.shape)
+
+    __call__ = forward

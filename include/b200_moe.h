@@ -341,6 +341,59 @@ int b200_ep_export(const void* ptr, void* handle /* B200_EP_HANDLE_BYTES */);
 int b200_ep_open(const void* handle, void** ptr);
 int b200_ep_close(void* ptr);
 
+/* ---- dense feed-forward operators: the residual stream with its norm, and non-expert projections, in bf16 / fp16 (with the pieces of their
+ * backward passes) and in FP8.  The reference computes these with torch (dsv41/model.py, Block and _swiglu :2337-2342); the clamps of the
+ * gated product are those of dsv41/fused.py:291-296.
+ * dtype: B200_BF16 / B200_FP16 (/ B200_FP32 for the norm); act: B200_ACT_*.  All sizes are element counts, *_ld are row strides in elements.
+ * Arguments are checked before anything is launched; M == 0 / rows == 0 is a valid call that writes nothing (weight and bias gradients: zeros).
+ *
+ * b200_add_rms_norm: s = x + residual (or x), y = s / sqrt(mean(s^2) + eps) * w (w NULL: 1), computed in fp32 from the unrounded sum; y and
+ *   sum [rows, dim] dense in `dtype`, either may be NULL;  q8 / sf (optional): y as e4m3 codes [rows, dim] with one E8M0 scale byte per 32
+ *   [rows, dim/32] (operands of b200_mx_grouped_gemm and b200_linear_act_q8), quantised from the fp32 y: scale = the smallest power of two
+ *   with max(|y|, 1e-4) / scale <= 448; needs dim % 32 == 0.  w in `dtype`, or fp32 with w_is_f32.  1 <= dim <= 16384, any strides.
+ * b200_add_rms_norm_bwd: ds (gradient of x and of residual) from gy [rows, dim] and gsum [rows, dim] (gradient of sum, or NULL), both dense;
+ *   dw [dim] in w's type (or NULL).  Workspace only for dw, 16-byte aligned.
+ *
+ * b200_linear_act: out[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + residual[M, N]; bias, residual, z may be NULL; z [M, N] receives the
+ *   pre-activation (what the backward pass needs).  x and w start on 16 bytes and their strides are multiples of 8 (b200_align_rows makes
+ *   such a copy of other tensors); everything else has any address and stride.
+ * b200_linear_act_bwd: dz = gy * act'(z) [M, N] (or NULL) and dbias [N] = its column sums (or NULL; needs the workspace).
+ * b200_gated_linear: out[M, inter] = act(min(g, limit)) * min(max(u, -limit), limit), [g | u] = x[M, K] w13[2 inter, K]^T, limit 0: no clamps;
+ *   gu [M, 2 inter] (or NULL): g and u for the backward pass, a clamped value stored as 1.0625 * limit with its sign.
+ * b200_gated_linear_bwd: dgu [M, 2 inter] from gy [M, inter] and that gu.
+ * b200_dense_product: out[M, N] = sum_k A(m, k) B(n, k), A(i, k) at base[i * ld + k], or base[k * ld + i] with *_mn != 0: the products of the
+ *   backward passes (dx = dz w: b_mn; dw = dz^T x: a_mn and b_mn) without transposed copies.  a_mn needs b_mn.  Alignment as b200_linear_act.
+ * b200_linear_act_q8: the projection with x as e4m3 [M, K] + E8M0 [M, K/32] and w as e4m3 [N, K] (natural k order) + E8M0 [ceil(N/32), s_cols];
+ *   bias, residual and out bf16.  K % 128 == 0, x8 and w8 16-byte aligned. */
+#define B200_BF16 0
+#define B200_FP16 1
+#define B200_FP32 2
+#define B200_ACT_NONE 0
+#define B200_ACT_RELU 1
+#define B200_ACT_SILU 2
+#define B200_ACT_GELU 3      /* z Phi(z) */
+#define B200_ACT_GELU_TANH 4
+int b200_add_rms_norm(const void* x, long long x_ld, const void* residual, long long r_ld, const void* w, int w_is_f32, int dtype, long long rows, int dim,
+                      float eps, void* y, void* sum, void* q8, void* sf, cudaStream_t stream);
+size_t b200_add_rms_norm_bwd_workspace_bytes(long long rows, int dim);
+int b200_add_rms_norm_bwd(const void* x, long long x_ld, const void* residual, long long r_ld, const void* w, int w_is_f32, int dtype, long long rows, int dim,
+                          float eps, const void* gy, const void* gsum, void* ds, void* dw, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+int b200_linear_act(const void* x, long long x_ld, const void* w, long long w_ld, int dtype, int M, int N, int K, const void* bias, int act, const void* residual,
+                    long long r_ld, void* out, long long out_ld, void* z, long long z_ld, cudaStream_t stream);
+size_t b200_linear_act_bwd_workspace_bytes(int M, int N);
+int b200_linear_act_bwd(const void* gy, long long gy_ld, const void* z, long long z_ld, int act, int dtype, int M, int N, void* dz, long long dz_ld, void* dbias,
+                        void* workspace, size_t workspace_bytes, cudaStream_t stream);
+int b200_gated_linear(const void* x, long long x_ld, const void* w13, long long w_ld, int dtype, int M, int inter, int K, int act, float limit, void* out,
+                      long long out_ld, void* gu, long long gu_ld, cudaStream_t stream);
+int b200_gated_linear_bwd(const void* gy, long long gy_ld, const void* gu, long long gu_ld, int act, float limit, int dtype, int M, int inter, void* dgu,
+                          long long dgu_ld, cudaStream_t stream);
+int b200_dense_product(const void* a, long long a_ld, int a_mn, const void* b, long long b_ld, int b_mn, int dtype, int M, int N, int K, void* out, long long out_ld,
+                       cudaStream_t stream);
+int b200_align_rows(const void* src, long long src_ld, void* dst, long long dst_ld, long long rows, int cols, cudaStream_t stream);
+size_t b200_linear_act_q8_workspace_bytes(int M, int N, int K);
+int b200_linear_act_q8(const void* x8, const void* xsf, const void* w8, const void* s8, int s_cols, int M, int N, int K, const void* bias, int act, const void* residual,
+                       long long r_ld, void* out, long long out_ld, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
 /* ---- device error word.  Every device-side wait of this library is bounded; one that runs out of time stores a non-zero
  * code instead of hanging.  Synchronises `stream`, returns the code in *code (0 = none) and clears it. */
 int b200_device_error(int* code, cudaStream_t stream);
