@@ -10,11 +10,12 @@
 
 namespace b200 {
 
-// dz = gy * act'(z) and the column sums of dz.  8 warps of a block share DZ_ROWS rows of 32 * VEC columns; the sums of a block's rows go to
+// dz = gy * act'(z) and the column sums of dz.  z arrives in fp32: in 16 bits its rounding would put an error of the size of the result's own
+// rounding into every gradient.  8 warps of a block share DZ_ROWS rows of 32 * VEC columns; the sums of a block's rows go to
 // part[block row][N] in fp32 (from the unrounded dz), added in block order afterwards.  Bound by HBM: gy and z in, dz out.
 constexpr int DZ_ROWS = 64;
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const T* __restrict__ z, long long z_ld, int act, int M, int N,
+__global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const float* __restrict__ z, long long z_ld, int act, int M, int N,
                                                       T* __restrict__ dz, long long dz_ld, float* __restrict__ part) {
     __shared__ float red[8][32 * VEC];
     pdl_wait();
@@ -31,7 +32,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, 
             load_vec<T, VEC>(gy + r * gy_ld + c, g);
             if (z) {
                 float v[VEC];
-                load_vec<T, VEC>(z + r * z_ld + c, v);
+                load_vec<float, VEC>(z + r * z_ld + c, v);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) g[i] *= act_bwd(act, v[i]).y;
             }
@@ -54,9 +55,9 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, 
 }
 
 // [dg | du] of the gated product from gy and the saved [g | u]: dg = gy u' act'(g') where the clamp let g through, du = gy act(g') where it
-// let u through (g', u': the clamped values).  Bound by HBM: 3 values in, 2 out per element of gy.
+// let u through (g', u': the clamped values).  g and u arrive in fp32 (as z above).  Bound by HBM: 10 bytes in, 4 out per element of gy.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const T* __restrict__ gu, long long gu_ld, int act, float limit, long long M,
+__global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const float* __restrict__ gu, long long gu_ld, int act, float limit, long long M,
                                                         int inter, T* __restrict__ dgu, long long dgu_ld) {
     pdl_wait();
     pdl_launch_dependents();
@@ -67,16 +68,16 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy
     const int c = (int)(i - r * per_row) * VEC;
     float d[VEC], g[VEC], u[VEC];
     load_vec<T, VEC>(gy + r * gy_ld + c, d);
-    load_vec<T, VEC>(gu + r * gu_ld + c, g);
-    load_vec<T, VEC>(gu + r * gu_ld + inter + c, u);
+    load_vec<float, VEC>(gu + r * gu_ld + c, g);
+    load_vec<float, VEC>(gu + r * gu_ld + inter + c, u);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
         bool pass_g = true, pass_u = true;
-        if (limit > 0.f) {  // clamped values were stored as 1.0625 limit (fgemm.cu); the others may have been rounded up to just above it
-            pass_g = !(g[k] > 1.03125f * limit);
-            pass_u = !(fabsf(u[k]) > 1.03125f * limit);
-            if (g[k] > limit) g[k] = limit;
-            if (fabsf(u[k]) > limit) u[k] = copysignf(limit, u[k]);
+        if (limit > 0.f) {
+            pass_g = !(g[k] > limit);
+            pass_u = !(fabsf(u[k]) > limit);
+            if (!pass_g) g[k] = limit;
+            if (!pass_u) u[k] = copysignf(limit, u[k]);
         }
         const float2 a = act_bwd(act, g[k]);
         g[k] = pass_g ? d[k] * u[k] * a.y : 0.f;
@@ -121,24 +122,24 @@ __global__ void __launch_bounds__(256) dequant_rows_kernel(const uint8_t* __rest
     store8<__nv_bfloat16>(out + r * K + c + 8, *reinterpret_cast<const float(*)[8]>(&v[8]));
 }
 
-static bool ok16(const void* p, long long ld) { return !((uintptr_t)p & 15) && ld % 8 == 0; }
+static bool ok16(const void* p, long long ld) { return !((uintptr_t)p & 15) && ld % 8 == 0; }  // rows start on 16 bytes (fp32: on 32)
 
 template <typename T>
-static int act_bwd_run(const void* gy, long long gy_ld, const void* z, long long z_ld, int act, int M, int N, void* dz, long long dz_ld, float* part, cudaStream_t stream) {
+static int act_bwd_run(const void* gy, long long gy_ld, const float* z, long long z_ld, int act, int M, int N, void* dz, long long dz_ld, float* part, cudaStream_t stream) {
     const bool vec = N % 8 == 0 && ok16(gy, gy_ld) && (!z || ok16(z, z_ld)) && (!dz || ok16(dz, dz_ld));
     const int w = vec ? 256 : 32;
     const dim3 grid((N + w - 1) / w, (M + DZ_ROWS - 1) / DZ_ROWS);
-    return (int)launch_pdl(vec ? act_bwd_kernel<T, 8> : act_bwd_kernel<T, 1>, grid, dim3(256), 0, stream, (const T*)gy, gy_ld, (const T*)z, z_ld, act, M, N, (T*)dz, dz_ld,
+    return (int)launch_pdl(vec ? act_bwd_kernel<T, 8> : act_bwd_kernel<T, 1>, grid, dim3(256), 0, stream, (const T*)gy, gy_ld, z, z_ld, act, M, N, (T*)dz, dz_ld,
                            part);
 }
 
 template <typename T>
-static int gated_bwd_run(const void* gy, long long gy_ld, const void* gu, long long gu_ld, int act, float limit, int M, int inter, void* dgu, long long dgu_ld,
+static int gated_bwd_run(const void* gy, long long gy_ld, const float* gu, long long gu_ld, int act, float limit, int M, int inter, void* dgu, long long dgu_ld,
                          cudaStream_t stream) {
     const bool vec = inter % 8 == 0 && ok16(gy, gy_ld) && ok16(gu, gu_ld) && ok16(dgu, dgu_ld);
     const long long threads = (long long)M * (vec ? inter / 8 : inter), blocks = (threads + 255) / 256;
     if (blocks > 0x7FFFFFFFll) return ERR_TOO_LARGE;
-    return (int)launch_pdl(vec ? gated_bwd_kernel<T, 8> : gated_bwd_kernel<T, 1>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)gy, gy_ld, (const T*)gu, gu_ld, act,
+    return (int)launch_pdl(vec ? gated_bwd_kernel<T, 8> : gated_bwd_kernel<T, 1>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)gy, gy_ld, gu, gu_ld, act,
                            limit, (long long)M, inter, (T*)dgu, dgu_ld);
 }
 
@@ -152,7 +153,7 @@ static int dense_check(int dtype, int act) {
 }
 
 extern "C" int b200_linear_act(const void* x, long long x_ld, const void* w, long long w_ld, int dtype, int M, int N, int K, const void* bias, int act,
-                               const void* residual, long long r_ld, void* out, long long out_ld, void* z, long long z_ld, cudaStream_t stream) {
+                               const void* residual, long long r_ld, void* out, long long out_ld, float* z, long long z_ld, cudaStream_t stream) {
     const int rc = dense_check(dtype, act);
     if (rc) return rc;
     if (M < 0 || N <= 0 || K <= 0) return ERR_BAD_SHAPE;
@@ -168,7 +169,7 @@ extern "C" int b200_linear_act(const void* x, long long x_ld, const void* w, lon
 }
 
 extern "C" int b200_gated_linear(const void* x, long long x_ld, const void* w13, long long w_ld, int dtype, int M, int inter, int K, int act, float limit, void* out,
-                                 long long out_ld, void* gu, long long gu_ld, cudaStream_t stream) {
+                                 long long out_ld, float* gu, long long gu_ld, cudaStream_t stream) {
     const int rc = dense_check(dtype, act);
     if (rc) return rc;
     if (M < 0 || inter <= 0 || inter > (1 << 29) || K <= 0 || !(limit >= 0.f)) return ERR_BAD_SHAPE;
@@ -203,7 +204,7 @@ extern "C" size_t b200_linear_act_bwd_workspace_bytes(int M, int N) {
     return (size_t)((M + DZ_ROWS - 1) / DZ_ROWS) * (size_t)N * sizeof(float);
 }
 
-extern "C" int b200_linear_act_bwd(const void* gy, long long gy_ld, const void* z, long long z_ld, int act, int dtype, int M, int N, void* dz, long long dz_ld, void* dbias,
+extern "C" int b200_linear_act_bwd(const void* gy, long long gy_ld, const float* z, long long z_ld, int act, int dtype, int M, int N, void* dz, long long dz_ld, void* dbias,
                                    void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     const int rc = dense_check(dtype, act);
     if (rc) return rc;
@@ -222,7 +223,7 @@ extern "C" int b200_linear_act_bwd(const void* gy, long long gy_ld, const void* 
     return column_sum(part, (M + DZ_ROWS - 1) / DZ_ROWS, N, dtype, dbias, stream);
 }
 
-extern "C" int b200_gated_linear_bwd(const void* gy, long long gy_ld, const void* gu, long long gu_ld, int act, float limit, int dtype, int M, int inter, void* dgu,
+extern "C" int b200_gated_linear_bwd(const void* gy, long long gy_ld, const float* gu, long long gu_ld, int act, float limit, int dtype, int M, int inter, void* dgu,
                                      long long dgu_ld, cudaStream_t stream) {
     const int rc = dense_check(dtype, act);
     if (rc) return rc;

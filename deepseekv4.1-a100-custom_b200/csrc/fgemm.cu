@@ -90,7 +90,7 @@ __device__ __forceinline__ void epilogue16(const FgParams& P, long long row, int
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i] = __uint_as_float(acc[i]);
     }
-    if (g.z_out) store16<T>(reinterpret_cast<T*>(g.z_out) + row * g.z_ld + col, P.vec_z, n, z);
+    if (g.z_out) store16<float>(g.z_out + row * g.z_ld + col, P.vec_z, n, z);
     if (g.act != ACT_NONE) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i] = act_fwd(g.act, z[i]);
@@ -113,16 +113,9 @@ __device__ __forceinline__ void epilogue16_dual(const FgParams& P, long long row
 #pragma unroll
     for (int i = 0; i < 16; ++i) { a[i] = __uint_as_float(ga[i]); b[i] = __uint_as_float(ua[i]); }
     if (g.z_out) {
-        // a clamped value is stored 1/16 above the limit, so that rounding cannot move a value across it: the backward pass takes what lies
-        // more than 1/32 above the limit as clamped
-        T* z = reinterpret_cast<T*>(g.z_out) + row * g.z_ld + col;
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = g.limit > 0.f && a[i] > g.limit ? 1.0625f * g.limit : a[i];
-        store16<T>(z, P.vec_z, n, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = g.limit > 0.f && fabsf(b[i]) > g.limit ? copysignf(1.0625f * g.limit, b[i]) : b[i];
-        store16<T>(z + g.inter, P.vec_z, n, v);
+        float* z = g.z_out + row * g.z_ld + col;
+        store16<float>(z, P.vec_z, n, a);
+        store16<float>(z + g.inter, P.vec_z, n, b);
     }
     if (g.limit > 0.f) {
 #pragma unroll
@@ -326,6 +319,7 @@ int fg_launch(const FgArgs& a, cudaStream_t stream) {
     if (a.dual && (a.N != 2 * a.inter || a.b.mn_major)) return ERR_BAD_SHAPE;
     if (((uintptr_t)a.a.base & 15) || ((uintptr_t)a.b.base & 15) || a.a.ld % 8 || a.b.ld % 8) return ERR_BAD_ALIGN;
     if (a.a.ld < (a.a.mn_major ? a.M : a.K) || a.b.ld < (a.b.mn_major ? a.N : a.K)) return ERR_BAD_SHAPE;
+    if (a.M <= FS_MAX_M && !a.a.mn_major && !a.b.mn_major) return fs_launch(a, stream);
     FgParams P{};
     P.g = a;
     auto vec = [](const void* p, long long ld) { return p && !((uintptr_t)p & 15) && ld % 8 == 0; };

@@ -18,7 +18,7 @@ struct FgArgs {
     FgOperand a, b;
     int M, N, K;             // N counts the rows of B (2 * inter with dual)
     int is_f16;              // 0: bf16, 1: fp16 (operands, bias, residual and outputs)
-    // epilogue: z = acc + bias;  out = act(z) + res;  z is stored too when z_out is given.
+    // epilogue: z = acc + bias;  out = act(z) + res;  z is stored too, in fp32, when z_out is given.
     // dual: B's rows are [gate | up], columns j and inter + j meet in one thread: out = act(min(g, limit)) * clamp(u, +-limit) (limit 0: no clamp);
     // z_out receives [g | u]
     int dual, inter;
@@ -29,11 +29,14 @@ struct FgArgs {
     long long res_ld;
     void* out;
     long long out_ld;
-    void* z_out;
+    float* z_out;
     long long z_ld;
 };
 
 int fg_launch(const FgArgs& a, cudaStream_t stream);
+// fstream.cu: the same for M <= FS_MAX_M, K-major operands
+constexpr int FS_MAX_M = 16;
+int fs_launch(const FgArgs& a, cudaStream_t stream);
 int fg_device_error(int* out);  // device error word (a wait that ran out of time), read and cleared
 
 }  // namespace b200

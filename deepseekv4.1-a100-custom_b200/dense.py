@@ -18,9 +18,38 @@ _PAIR = (torch.bfloat16, torch.float16)
 
 
 # ------------------------------------------------------------------ marshalling
+# The small calls of a decode step are bound by the host: addresses go to ctypes as plain integers, the stream is read without building a
+# Stream object, and the device is switched only when it is not the current one (23 us -> 12 us for a one-row norm).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(name: str, dev: torch.device, *args) -> None:
+    fn = getattr(L.lib(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc:
+        L.check(rc, name)
+
+
+def _size(name: str, dev: torch.device, *args) -> int:
+    """A *_workspace_bytes function, which sizes for the current device."""
+    with torch.cuda.device(dev):
+        return getattr(L.lib(), name)(*args)
+
+
+def _ptr(t) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., D] as rows [R, D] with a unit inner stride and rows that do not overlap (a copy only where the strides do not allow a view)."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         t = t.contiguous()
     return t
@@ -38,26 +67,34 @@ def _tma_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """Rows as the tensor-core kernels fetch them: 16-byte aligned base, stride a multiple of 8 elements; other rows are copied once."""
     t = _rows(t)
     r, d = t.shape
-    if t.data_ptr() % 16 == 0 and (r == 1 or t.stride(0) % 8 == 0):
-        return t, t.stride(0) if r > 1 else _pitch(d)
+    if t.data_ptr() % 16 == 0:
+        if r == 1:
+            return t, _pitch(d)
+        ld = t.stride(0)
+        if ld % 8 == 0:
+            return t, ld
     ld = _pitch(d)
     out = torch.empty(r, ld, device=t.device, dtype=t.dtype)
-    L.check(L.lib().b200_align_rows(L.ptr(t), _ld(t), L.ptr(out), ld, r, d, L.stream_of(t.device)), "b200_align_rows")
+    _call("b200_align_rows", t.device, t.data_ptr(), _ld(t), out.data_ptr(), ld, r, d)
     return out[:, :d], ld
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K) -> torch.Tensor:
     out = torch.empty(M, N, device=a.device, dtype=a.dtype)
-    L.check(L.lib().b200_dense_product(L.ptr(a), a_ld, a_mn, L.ptr(b), b_ld, b_mn, L.DTYPES[a.dtype], M, N, K, L.ptr(out), N, L.stream_of(a.device)), "b200_dense_product")
+    _call("b200_dense_product", a.device, a.data_ptr(), a_ld, a_mn, b.data_ptr(), b_ld, b_mn, L.DTYPES[a.dtype], M, N, K, out.data_ptr(), N)
     return out
 
 
-def _empty_scratch(nbytes: int, device) -> torch.Tensor:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _scratch(nbytes: int, device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 # ------------------------------------------------------------------ residual addition + rms norm
@@ -74,9 +111,9 @@ def _norm_args(x, residual, weight, eps):
 
 def _norm_forward(x, residual, weight, eps, y, s, q8, sf):
     """x, residual: 2-D rows; weight contiguous."""
-    L.check(L.lib().b200_add_rms_norm(L.ptr(x), _ld(x), L.ptr(residual), _ld(residual) if residual is not None else 0, L.ptr(weight),
-                                      int(weight is not None and weight.dtype == torch.float32), L.DTYPES[x.dtype], x.shape[0], x.shape[1], float(eps), L.ptr(y), L.ptr(s),
-                                      L.ptr(q8), L.ptr(sf), L.stream_of(x.device)), "b200_add_rms_norm")
+    rows, D = x.shape
+    _call("b200_add_rms_norm", x.device, x.data_ptr(), _ld(x), _ptr(residual), 0 if residual is None else _ld(residual), _ptr(weight),
+          weight is not None and weight.dtype is torch.float32, L.DTYPES[x.dtype], rows, D, eps, _ptr(y), _ptr(s), _ptr(q8), _ptr(sf))
 
 
 class _AddRmsNorm(torch.autograd.Function):
@@ -86,8 +123,7 @@ class _AddRmsNorm(torch.autograd.Function):
         y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
         s = torch.empty_like(y) if residual is not None else None
         wc = weight.contiguous() if weight is not None else None
-        with torch.cuda.device(x.device):
-            _norm_forward(x2, r2, wc, eps, y, s, None, None)
+        _norm_forward(x2, r2, wc, eps, y, s, None, None)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x2, r2, wc)
         ctx.eps, ctx.shape = eps, x.shape
@@ -99,21 +135,17 @@ class _AddRmsNorm(torch.autograd.Function):
         x, r, w = ctx.saved_tensors
         need_x, need_r, need_w, _ = ctx.needs_input_grad
         if gy is None:  # the normed output was not used
-            dw = torch.zeros_like(w) if need_w else None
-            return gs if need_x else None, gs if need_r else None, dw, None
+            return gs if need_x else None, gs if need_r else None, torch.zeros_like(w) if need_w else None, None
         dev = x.device
         gy = gy.contiguous()
         gs = gs.contiguous() if gs is not None else None
         rows, D = x.shape
         ds = torch.empty(ctx.shape, device=dev, dtype=x.dtype)
         dw = torch.empty_like(w) if need_w else None
-        with torch.cuda.device(dev):
-            lib = L.lib()
-            nb = lib.b200_add_rms_norm_bwd_workspace_bytes(rows, D) if need_w else 0
-            ws = _empty_scratch(nb, dev) if nb else None
-            L.check(lib.b200_add_rms_norm_bwd(L.ptr(x), _ld(x), L.ptr(r), _ld(r) if r is not None else 0, L.ptr(w), int(w is not None and w.dtype == torch.float32),
-                                              L.DTYPES[x.dtype], rows, D, float(ctx.eps), L.ptr(gy), L.ptr(gs), L.ptr(ds), L.ptr(dw), L.ptr(ws), nb, L.stream_of(dev)),
-                    "b200_add_rms_norm_bwd")
+        nb = _size("b200_add_rms_norm_bwd_workspace_bytes", dev, rows, D) if need_w else 0
+        ws = _scratch(nb, dev)
+        _call("b200_add_rms_norm_bwd", dev, x.data_ptr(), _ld(x), _ptr(r), 0 if r is None else _ld(r), _ptr(w), w is not None and w.dtype is torch.float32, L.DTYPES[x.dtype],
+              rows, D, ctx.eps, gy.data_ptr(), _ptr(gs), ds.data_ptr(), _ptr(dw), _ptr(ws), nb)
         return ds if need_x else None, ds if need_r else None, dw, None
 
 
@@ -127,8 +159,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: 
     x2, r2 = _rows(x), _rows(residual) if residual is not None else None
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     s = torch.empty_like(y) if residual is not None else None
-    with torch.cuda.device(x.device):
-        _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, eps, y, s, None, None)
+    _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, float(eps), y, s, None, None)
     return y, (s if residual is not None else x)
 
 
@@ -145,8 +176,7 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None = None, we
     sf = torch.empty(rows, D // 32, device=dev, dtype=torch.uint8)
     s = torch.empty(x.shape, device=dev, dtype=x.dtype) if residual is not None else None
     y = torch.empty(x.shape, device=dev, dtype=x.dtype) if want_y else None
-    with torch.cuda.device(dev):
-        _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, eps, y, s, q8, sf)
+    _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, float(eps), y, s, q8, sf)
     s = s if residual is not None else x
     return (q8, sf, s, y) if want_y else (q8, sf, s)
 
@@ -155,24 +185,22 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None = None, we
 def _linear_forward(x, x_ld, w, w_ld, bias, act, residual, out, z, z_ld):
     M, K = x.shape
     N = w.shape[0]
-    r_ld = _ld(residual) if residual is not None else 0
-    L.check(L.lib().b200_linear_act(L.ptr(x), x_ld, L.ptr(w), w_ld, L.DTYPES[x.dtype], M, N, K, L.ptr(bias), act, L.ptr(residual), r_ld, L.ptr(out), N, L.ptr(z), z_ld,
-                                    L.stream_of(x.device)), "b200_linear_act")
+    _call("b200_linear_act", x.device, x.data_ptr(), x_ld, w.data_ptr(), w_ld, L.DTYPES[x.dtype], M, N, K, _ptr(bias), act, _ptr(residual),
+          0 if residual is None else _ld(residual), out.data_ptr(), N, _ptr(z), z_ld)
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, act, residual):
-        M_shape, N = x.shape[:-1], w.shape[0]
-        with torch.cuda.device(x.device):
-            x2, x_ld = _tma_rows(x)
-            w2, w_ld = _tma_rows(w)
-            r2 = _rows(residual) if residual is not None else None
-            b = bias.contiguous() if bias is not None else None
-            out = torch.empty(*M_shape, N, device=x.device, dtype=x.dtype)
-            z_ld = _pitch(N)
-            z = torch.empty(x2.shape[0], z_ld, device=x.device, dtype=x.dtype) if act else None
-            _linear_forward(x2, x_ld, w2, w_ld, b, act, r2, out, z, z_ld)
+        N = w.shape[0]
+        x2, x_ld = _tma_rows(x)
+        w2, w_ld = _tma_rows(w)
+        r2 = _rows(residual) if residual is not None else None
+        b = bias.contiguous() if bias is not None else None
+        out = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
+        z_ld = _pitch(N)
+        z = torch.empty(x2.shape[0], z_ld, device=x.device, dtype=torch.float32) if act else None
+        _linear_forward(x2, x_ld, w2, w_ld, b, act, r2, out, z, z_ld)
         ctx.save_for_backward(x2, w2, z)
         ctx.x_ld, ctx.w_ld, ctx.act, ctx.x_shape = x_ld, w_ld, act, x.shape
         return out
@@ -182,27 +210,26 @@ class _LinearAct(torch.autograd.Function):
     def backward(ctx, gy):
         x, w, z = ctx.saved_tensors
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
-        (M, K), N, dev, lib = x.shape, w.shape[0], x.device, L.lib()
+        (M, K), N, dev = x.shape, w.shape[0], x.device
         g2 = _rows(gy)
         dx = dw = db = None
-        with torch.cuda.device(dev):
-            if need_b:
-                db = torch.empty(N, device=dev, dtype=x.dtype)
-            dz, dz_ld = g2, _ld(g2)
-            if (need_x or need_w) and (ctx.act or N % 8):
-                dz_ld = _pitch(N)
-                dz = torch.empty(M, dz_ld, device=dev, dtype=x.dtype)
-            if dz is not g2 or need_b:
-                nb = lib.b200_linear_act_bwd_workspace_bytes(M, N) if need_b else 0
-                ws = _empty_scratch(nb, dev) if nb else None
-                L.check(lib.b200_linear_act_bwd(L.ptr(g2), _ld(g2), L.ptr(z), _pitch(N) if z is not None else 0, ctx.act, L.DTYPES[x.dtype], M, N,
-                                                L.ptr(dz) if dz is not g2 else None, dz_ld, L.ptr(db), L.ptr(ws), nb, L.stream_of(dev)), "b200_linear_act_bwd")
-            if (need_x or need_w) and dz is g2:
-                dz, dz_ld = _tma_rows(g2)
-            if need_x:
-                dx = _product(dz, dz_ld, 0, w, ctx.w_ld, 1, M, K, N).view(ctx.x_shape)
-            if need_w:
-                dw = _product(dz, dz_ld, 1, x, ctx.x_ld, 1, N, K, M) if M else torch.zeros(N, K, device=dev, dtype=x.dtype)
+        if need_b:
+            db = torch.empty(N, device=dev, dtype=x.dtype)
+        dz, dz_ld = g2, _ld(g2)
+        if (need_x or need_w) and (ctx.act or N % 8):
+            dz_ld = _pitch(N)
+            dz = torch.empty(M, dz_ld, device=dev, dtype=x.dtype)
+        if dz is not g2 or need_b:
+            nb = _size("b200_linear_act_bwd_workspace_bytes", dev, M, N) if need_b else 0
+            ws = _scratch(nb, dev)
+            _call("b200_linear_act_bwd", dev, g2.data_ptr(), _ld(g2), _ptr(z), _pitch(N), ctx.act, L.DTYPES[x.dtype], M, N, dz.data_ptr() if dz is not g2 else None, dz_ld,
+                  _ptr(db), _ptr(ws), nb)
+        if (need_x or need_w) and dz is g2:
+            dz, dz_ld = _tma_rows(g2)
+        if need_x:
+            dx = _product(dz, dz_ld, 0, w, ctx.w_ld, 1, M, K, N).view(ctx.x_shape)
+        if need_w:
+            dw = _product(dz, dz_ld, 1, x, ctx.x_ld, 1, N, K, M) if M else torch.zeros(N, K, device=dev, dtype=x.dtype)
         return dx, dw, db, None, gy if need_r else None
 
 
@@ -214,7 +241,8 @@ def _act_code(act) -> int:
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
     """act(x w^T + bias) + residual: x [..., K], w [N, K], bias [N], residual [..., N], all bf16 or all fp16; act None, "relu", "silu", "gelu"
     (z Phi(z)) or "gelu_tanh".  fp32 accumulation, one rounding at the end.  Any K, N and number of rows; rows of x or w that do not start on
-    16 bytes (a K that is no multiple of 8, an odd slice) are copied first.  Differentiable in x, w, bias and residual."""
+    16 bytes (a K that is no multiple of 8, an odd slice) are copied first.  Differentiable in x, w, bias and residual; with an activation a call
+    that needs a gradient also keeps the pre-activation (N fp32 values per row)."""
     L.require_cuda(x, w, bias, residual)
     code = _act_code(act)
     assert x.dtype in _PAIR and w.dtype == x.dtype and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
@@ -225,10 +253,9 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     if _wants_grad(x, w, bias, residual):
         return _LinearAct.apply(x, w, bias, code, residual)
     out = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
-    with torch.cuda.device(x.device):
-        x2, x_ld = _tma_rows(x)
-        w2, w_ld = _tma_rows(w)
-        _linear_forward(x2, x_ld, w2, w_ld, bias.contiguous() if bias is not None else None, code, _rows(residual) if residual is not None else None, out, None, 0)
+    x2, x_ld = _tma_rows(x)
+    w2, w_ld = _tma_rows(w)
+    _linear_forward(x2, x_ld, w2, w_ld, bias.contiguous() if bias is not None else None, code, _rows(residual) if residual is not None else None, out, None, 0)
     return out
 
 
@@ -249,12 +276,11 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
     x8, xsf, w8, s8 = (t.contiguous() for t in (x8, xsf, w8, s8))
     r2 = _rows(residual) if residual is not None else None
     out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
-    with torch.cuda.device(dev):
-        lib = L.lib()
-        nb = lib.b200_linear_act_q8_workspace_bytes(M, N, K)
-        ws = _empty_scratch(nb, dev) if nb else None
-        L.check(lib.b200_linear_act_q8(L.ptr(x8), L.ptr(xsf), L.ptr(w8), L.ptr(s8), s8.shape[1], M, N, K, L.ptr(bias.contiguous() if bias is not None else None), code,
-                                       L.ptr(r2), _ld(r2) if r2 is not None else 0, L.ptr(out), N, L.ptr(ws), nb, L.stream_of(dev)), "b200_linear_act_q8")
+    b = bias.contiguous() if bias is not None else None
+    nb = _size("b200_linear_act_q8_workspace_bytes", dev, M, N, K)
+    ws = _scratch(nb, dev)
+    _call("b200_linear_act_q8", dev, x8.data_ptr(), xsf.data_ptr(), w8.data_ptr(), s8.data_ptr(), s8.shape[1], M, N, K, _ptr(b), code, _ptr(r2), 0 if r2 is None else _ld(r2),
+          out.data_ptr(), N, _ptr(ws), nb)
     return out
 
 
@@ -262,21 +288,19 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
 def _gated_forward(x, x_ld, w, w_ld, act, limit, out, gu, gu_ld):
     M, K = x.shape
     inter = w.shape[0] // 2
-    L.check(L.lib().b200_gated_linear(L.ptr(x), x_ld, L.ptr(w), w_ld, L.DTYPES[x.dtype], M, inter, K, act, float(limit), L.ptr(out), inter, L.ptr(gu), gu_ld,
-                                      L.stream_of(x.device)), "b200_gated_linear")
+    _call("b200_gated_linear", x.device, x.data_ptr(), x_ld, w.data_ptr(), w_ld, L.DTYPES[x.dtype], M, inter, K, act, limit, out.data_ptr(), inter, _ptr(gu), gu_ld)
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, act, limit):
         inter = w13.shape[0] // 2
-        with torch.cuda.device(x.device):
-            x2, x_ld = _tma_rows(x)
-            w2, w_ld = _tma_rows(w13)
-            out = torch.empty(*x.shape[:-1], inter, device=x.device, dtype=x.dtype)
-            gu_ld = _pitch(2 * inter)
-            gu = torch.empty(x2.shape[0], gu_ld, device=x.device, dtype=x.dtype)
-            _gated_forward(x2, x_ld, w2, w_ld, act, limit, out, gu, gu_ld)
+        x2, x_ld = _tma_rows(x)
+        w2, w_ld = _tma_rows(w13)
+        out = torch.empty(*x.shape[:-1], inter, device=x.device, dtype=x.dtype)
+        gu_ld = _pitch(2 * inter)
+        gu = torch.empty(x2.shape[0], gu_ld, device=x.device, dtype=torch.float32)
+        _gated_forward(x2, x_ld, w2, w_ld, act, limit, out, gu, gu_ld)
         ctx.save_for_backward(x2, w2, gu)
         ctx.x_ld, ctx.w_ld, ctx.act, ctx.limit, ctx.x_shape = x_ld, w_ld, act, limit, x.shape
         return out
@@ -290,21 +314,19 @@ class _GatedLinear(torch.autograd.Function):
         g2 = _rows(gy)
         gu_ld = _pitch(n2)
         dx = dw = None
-        with torch.cuda.device(dev):
-            dgu = torch.empty(M, gu_ld, device=dev, dtype=x.dtype)
-            L.check(L.lib().b200_gated_linear_bwd(L.ptr(g2), _ld(g2), L.ptr(gu), gu_ld, ctx.act, float(ctx.limit), L.DTYPES[x.dtype], M, n2 // 2, L.ptr(dgu), gu_ld,
-                                                  L.stream_of(dev)), "b200_gated_linear_bwd")
-            if need_x:
-                dx = _product(dgu, gu_ld, 0, w, ctx.w_ld, 1, M, K, n2).view(ctx.x_shape)
-            if need_w:
-                dw = _product(dgu, gu_ld, 1, x, ctx.x_ld, 1, n2, K, M) if M else torch.zeros(n2, K, device=dev, dtype=x.dtype)
+        dgu = torch.empty(M, gu_ld, device=dev, dtype=x.dtype)
+        _call("b200_gated_linear_bwd", dev, g2.data_ptr(), _ld(g2), gu.data_ptr(), gu_ld, ctx.act, ctx.limit, L.DTYPES[x.dtype], M, n2 // 2, dgu.data_ptr(), gu_ld)
+        if need_x:
+            dx = _product(dgu, gu_ld, 0, w, ctx.w_ld, 1, M, K, n2).view(ctx.x_shape)
+        if need_w:
+            dw = _product(dgu, gu_ld, 1, x, ctx.x_ld, 1, n2, K, M) if M else torch.zeros(n2, K, device=dev, dtype=x.dtype)
         return dx, dw, None, None
 
 
 def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", limit: float = 0.0) -> torch.Tensor:
     """act(min(g, limit)) * min(max(u, -limit), limit) with [g | u] = x w13^T, both projections and the product in one kernel: x [..., K], w13
     [2 * inter, K] (gate rows, then up rows: the layout of the expert weights), both bf16 or both fp16 -> [..., inter].  limit 0: no clamps.
-    Differentiable in x and w13; a call that needs a gradient also keeps g and u (2 * inter values per row)."""
+    Differentiable in x and w13; a call that needs a gradient also keeps g and u (2 * inter fp32 values per row)."""
     L.require_cuda(x, w13)
     code = _act_code(act)
     assert x.dtype in _PAIR and w13.dtype == x.dtype and w13.dim() == 2, "x and w13 must be both bfloat16 or both float16, w13 [2 * inter, K]"
@@ -314,10 +336,9 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", l
     if _wants_grad(x, w13):
         return _GatedLinear.apply(x, w13, code, float(limit))
     out = torch.empty(*x.shape[:-1], n2 // 2, device=x.device, dtype=x.dtype)
-    with torch.cuda.device(x.device):
-        x2, x_ld = _tma_rows(x)
-        w2, w_ld = _tma_rows(w13)
-        _gated_forward(x2, x_ld, w2, w_ld, code, limit, out, None, 0)
+    x2, x_ld = _tma_rows(x)
+    w2, w_ld = _tma_rows(w13)
+    _gated_forward(x2, x_ld, w2, w_ld, code, float(limit), out, None, 0)
     return out
 
 

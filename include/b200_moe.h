@@ -354,12 +354,12 @@ int b200_ep_close(void* ptr);
  * b200_add_rms_norm_bwd: ds (gradient of x and of residual) from gy [rows, dim] and gsum [rows, dim] (gradient of sum, or NULL), both dense;
  *   dw [dim] in w's type (or NULL).  Workspace only for dw, 16-byte aligned.
  *
- * b200_linear_act: out[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + residual[M, N]; bias, residual, z may be NULL; z [M, N] receives the
+ * b200_linear_act: out[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + residual[M, N]; bias, residual, z may be NULL; z fp32 [M, N] receives the
  *   pre-activation (what the backward pass needs).  x and w start on 16 bytes and their strides are multiples of 8 (b200_align_rows makes
  *   such a copy of other tensors); everything else has any address and stride.
  * b200_linear_act_bwd: dz = gy * act'(z) [M, N] (or NULL) and dbias [N] = its column sums (or NULL; needs the workspace).
  * b200_gated_linear: out[M, inter] = act(min(g, limit)) * min(max(u, -limit), limit), [g | u] = x[M, K] w13[2 inter, K]^T, limit 0: no clamps;
- *   gu [M, 2 inter] (or NULL): g and u for the backward pass, a clamped value stored as 1.0625 * limit with its sign.
+ *   gu fp32 [M, 2 inter] (or NULL): g and u, unclamped, for the backward pass.
  * b200_gated_linear_bwd: dgu [M, 2 inter] from gy [M, inter] and that gu.
  * b200_dense_product: out[M, N] = sum_k A(m, k) B(n, k), A(i, k) at base[i * ld + k], or base[k * ld + i] with *_mn != 0: the products of the
  *   backward passes (dx = dz w: b_mn; dw = dz^T x: a_mn and b_mn) without transposed copies.  a_mn needs b_mn.  Alignment as b200_linear_act.
@@ -379,13 +379,13 @@ size_t b200_add_rms_norm_bwd_workspace_bytes(long long rows, int dim);
 int b200_add_rms_norm_bwd(const void* x, long long x_ld, const void* residual, long long r_ld, const void* w, int w_is_f32, int dtype, long long rows, int dim,
                           float eps, const void* gy, const void* gsum, void* ds, void* dw, void* workspace, size_t workspace_bytes, cudaStream_t stream);
 int b200_linear_act(const void* x, long long x_ld, const void* w, long long w_ld, int dtype, int M, int N, int K, const void* bias, int act, const void* residual,
-                    long long r_ld, void* out, long long out_ld, void* z, long long z_ld, cudaStream_t stream);
+                    long long r_ld, void* out, long long out_ld, float* z, long long z_ld, cudaStream_t stream);
 size_t b200_linear_act_bwd_workspace_bytes(int M, int N);
-int b200_linear_act_bwd(const void* gy, long long gy_ld, const void* z, long long z_ld, int act, int dtype, int M, int N, void* dz, long long dz_ld, void* dbias,
+int b200_linear_act_bwd(const void* gy, long long gy_ld, const float* z, long long z_ld, int act, int dtype, int M, int N, void* dz, long long dz_ld, void* dbias,
                         void* workspace, size_t workspace_bytes, cudaStream_t stream);
 int b200_gated_linear(const void* x, long long x_ld, const void* w13, long long w_ld, int dtype, int M, int inter, int K, int act, float limit, void* out,
-                      long long out_ld, void* gu, long long gu_ld, cudaStream_t stream);
-int b200_gated_linear_bwd(const void* gy, long long gy_ld, const void* gu, long long gu_ld, int act, float limit, int dtype, int M, int inter, void* dgu,
+                      long long out_ld, float* gu, long long gu_ld, cudaStream_t stream);
+int b200_gated_linear_bwd(const void* gy, long long gy_ld, const float* gu, long long gu_ld, int act, float limit, int dtype, int M, int inter, void* dgu,
                           long long dgu_ld, cudaStream_t stream);
 int b200_dense_product(const void* a, long long a_ld, int a_mn, const void* b, long long b_ld, int b_mn, int dtype, int M, int N, int K, void* out, long long out_ld,
                        cudaStream_t stream);
