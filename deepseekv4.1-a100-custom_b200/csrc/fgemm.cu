@@ -1,10 +1,12 @@
 // 16-bit GEMM on the 5th-generation tensor cores (tcgen05.mma.kind::f16, TMA, TMEM) with the epilogues of the dense operators: bias,
 // activation and residual, or the gated product of two projections.
 //
-// Persistent CTAs, one per SM, walk 128 x BN output tiles.  Warp roles:
+// Persistent CTAs, one per SM, walk the output tiles; with CG = 2 a pair of SMs (a cluster of two CTAs) shares a tile of 256 x BN
+// (tcgen05 cta_group::2): each SM fetches its own 128 rows of A and half of the rows of B, so a k block costs 16 + BN/16 KB of shared memory
+// traffic per 128 x BN of results where a lone SM needs 16 + BN/8.  Warp roles:
 //   warp 0      TMA producer: 64-deep k blocks of both operands into a ring of shared-memory stages (128-byte swizzle)
-//   warp 1      one thread issues the MMAs; the accumulators live in TMEM, two buffers, so that the epilogue of a tile runs under the
-//               MMAs of the next
+//   warp 1      one thread (of the first CTA of a pair) issues the MMAs; the accumulators live in TMEM, two buffers, so that the epilogue of
+//               a tile runs under the MMAs of the next
 //   warps 4-11  epilogue: a thread owns one output row (TMEM lane) and half of the tile's columns
 // Every wait is bounded; one that runs out of time records a code in a device error word and the CTA runs to its end.
 #include "fgemm.cuh"
@@ -18,9 +20,15 @@ namespace b200 {
 __device__ int g_fg_error = 0;
 
 constexpr int FG_THREADS = 384;
-constexpr int FG_BM = 128, FG_BK = 64;
-constexpr int FG_MAX_STAGES = 6;
-constexpr int FG_GROUP_M = 8;  // row tiles that are walked together down the columns: their A tiles stay in L2 while B passes once
+constexpr int FG_BM = 128, FG_BK = 64;  // rows of A per CTA, depth of a k block
+constexpr int FG_GROUP_M = 8;           // row tiles that are walked together down the columns: their A tiles stay in L2 while B passes once
+constexpr int FG_SMEM = 192 * 1024;     // ring of stages
+
+template <int CG, int BN>
+struct FgShape {
+    static constexpr uint32_t A_BYTES = FG_BM * FG_BK * 2, B_ROWS = BN / CG, B_BYTES = B_ROWS * FG_BK * 2, STAGE = A_BYTES + B_BYTES;
+    static constexpr int NS = FG_SMEM / STAGE;
+};
 
 struct FgParams {
     FgArgs g;
@@ -28,11 +36,62 @@ struct FgParams {
     int vec_out, vec_res, vec_z, vec_bias;  // rows allow 16-byte accesses
 };
 
+template <int CG>
 __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if constexpr (CG == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(adesc), "l"(bdesc),
+                     "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(adesc), "l"(bdesc),
+                     "r"(idesc), "r"(accumulate)
+                     : "memory");
+}
+// the MMAs issued so far, when done, arrive on this barrier (CG = 2: on the barrier at the same place in both CTAs of the pair)
+template <int CG>
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else
+        tc_commit(bar);
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc_all(uint32_t smem_dst) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_dst) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tmem_alloc(smem_dst, 512);
+        tmem_relinquish();
+    }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_dealloc_all(uint32_t taddr) {
+    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+    else tmem_dealloc(taddr, 512);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// address of the same shared-memory location in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// a box into this CTA's shared memory, its bytes counted on a barrier that may lie in the other CTA of the pair
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(tm), "r"(x), "r"(y),
+                 "r"(cluster_bar)
+                 : "memory");
 }
 
 // MN-major operand tile with the 128-byte swizzle: boxes of 64 rows-of-the-operand x 64 k, [box][k][64]; 8 k are 1024 bytes apart (stride
@@ -129,15 +188,16 @@ __device__ __forceinline__ void epilogue16_dual(const FgParams& P, long long row
     store16<T>(reinterpret_cast<T*>(g.out) + row * g.out_ld + col, P.vec_out, n, a);
 }
 
-template <typename T, int BN, bool A_MN, bool B_MN>
+template <typename T, int CG, int BN, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P, const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b) {
-    constexpr uint32_t A_BYTES = FG_BM * FG_BK * 2, B_BYTES = BN * FG_BK * 2, STAGE = A_BYTES + B_BYTES;
-    constexpr int NS = BN == 256 ? 4 : 6;
+    using S = FgShape<CG, BN>;
+    constexpr int NS = S::NS;
     extern __shared__ __align__(1024) uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long bars[2 * NS + 4];  // full[s], empty[s], acc_full[2], acc_empty[2]
     __shared__ uint32_t tmem_base_sh;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;  // the first CTA of a pair issues the MMAs; full[] and acc_empty[] are used there
     uint8_t* ring = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     auto bar_full = [&](int s) { return smem_u32(&bars[s]); };
     auto bar_empty = [&](int s) { return smem_u32(&bars[NS + s]); };
@@ -146,55 +206,60 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < NS; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(bar_acc_full(b), 1); mbar_init(bar_acc_empty(b), 8); }
+        for (int b = 0; b < 2; ++b) { mbar_init(bar_acc_full(b), 1); mbar_init(bar_acc_empty(b), 8 * CG); }
         mbar_fence_init();
     }
-    if (warp == 1) {
-        tmem_alloc(smem_u32(&tmem_base_sh), 512);
-        tmem_relinquish();
-    }
+    if (warp == 1) tmem_alloc_all<CG>(smem_u32(&tmem_base_sh));
     tc_fence_before();
-    __syncthreads();
+    __syncwarp();
+    if constexpr (CG == 2) cluster_sync();
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_sh;
     pdl_wait();
     pdl_launch_dependents();
     const FgArgs& g = P.g;
-    const int tiles = P.m_tiles * P.n_tiles;
+    const int tiles = P.m_tiles * P.n_tiles, first = blockIdx.x / CG, step = gridDim.x / CG;
 
     if (warp == 0) {
         if (lane == 0) {
             tma_prefetch_desc(&tm_a);
             tma_prefetch_desc(&tm_b);
             uint32_t n = 0;
-            for (int i = blockIdx.x; i < tiles && !abort_flag; i += gridDim.x) {
+            for (int i = first; i < tiles && !abort_flag; i += step) {
                 const Tile t = tile_at(i, P.m_tiles, P.n_tiles);
-                const int m0 = t.m * FG_BM;
-                // the two halves of the B tile: consecutive rows, or gate rows and up rows
-                const int n0 = g.dual ? t.n * (BN / 2) : t.n * BN, n1 = g.dual ? g.inter + n0 : n0 + BN / 2;
+                const int m0 = (t.m * CG + (int)rank) * FG_BM;
+                // the two halves of the B tile: consecutive rows, or gate rows and up rows; a CTA of a pair loads one of them
+                const int h0 = g.dual ? t.n * (BN / 2) : t.n * BN, h1 = g.dual ? g.inter + h0 : h0 + BN / 2;
+                const int n0 = rank ? h1 : h0;
                 for (int kb = 0; kb < P.k_blocks; ++kb, ++n) {
                     const uint32_t s = n % NS, ph = (n / NS) & 1;
                     if (!mbar_wait(bar_empty(s), ph ^ 1, &abort_flag, &g_fg_error, 1)) break;
-                    mbar_expect_tx(bar_full(s), STAGE);
-                    const uint32_t da = smem_u32(ring + (size_t)s * STAGE), db = da + A_BYTES;
+                    const uint32_t da = smem_u32(ring + (size_t)s * S::STAGE), db = da + S::A_BYTES;
                     const int k0 = kb * FG_BK;
+                    if (rank == 0) mbar_expect_tx(bar_full(s), CG * S::STAGE);
+                    const uint32_t bar = CG == 2 ? map_rank(bar_full(s), 0) : bar_full(s);
+                    auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
+                        if constexpr (CG == 2) tma_load_2d_pair(dst, tm, x, y, bar);
+                        else tma_load_2d(dst, tm, x, y, bar);
+                    };
                     if constexpr (A_MN) {
 #pragma unroll
-                        for (int q = 0; q < FG_BM / 64; ++q) tma_load_2d(da + q * 8192, &tm_a, m0 + q * 64, k0, bar_full(s));
+                        for (int q = 0; q < FG_BM / 64; ++q) load(da + q * 8192, &tm_a, m0 + q * 64, k0);
                     } else {
-                        tma_load_2d(da, &tm_a, k0, m0, bar_full(s));
+                        load(da, &tm_a, k0, m0);
                     }
                     if constexpr (B_MN) {
 #pragma unroll
-                        for (int q = 0; q < BN / 64; ++q) tma_load_2d(db + q * 8192, &tm_b, n0 + q * 64, k0, bar_full(s));
+                        for (int q = 0; q < (int)S::B_ROWS / 64; ++q) load(db + q * 8192, &tm_b, n0 + q * 64, k0);
                     } else {
-                        tma_load_2d(db, &tm_b, k0, n0, bar_full(s));
-                        tma_load_2d(db + B_BYTES / 2, &tm_b, k0, n1, bar_full(s));
+                        load(db, &tm_b, k0, n0);
+                        if constexpr (CG == 1) load(db + S::B_BYTES / 2, &tm_b, k0, h1);
                     }
                 }
             }
-            // every load issued above must have landed before the CTA may exit
-            for (int k = 0; k < NS && k < (int)n; ++k) {
+            // every load issued above must have landed before the CTA may exit (the second CTA of a pair is kept by the cluster barrier below)
+            for (int k = 0; rank == 0 && k < NS && k < (int)n; ++k) {
                 const uint32_t m = n - 1 - k, s = m % NS, ph = (m / NS) & 1;
                 const unsigned long long t0 = global_timer_ns();
                 while (!mbar_test(bar_full(s), ph))
@@ -202,10 +267,10 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = f16_idesc(g.is_f16, A_MN, B_MN, FG_BM, BN);
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = f16_idesc(g.is_f16, A_MN, B_MN, FG_BM * CG, BN);
             uint32_t n = 0, it = 0;
-            for (int i = blockIdx.x; i < tiles && !abort_flag; i += gridDim.x, ++it) {
+            for (int i = first; i < tiles && !abort_flag; i += step, ++it) {
                 const uint32_t buf = it & 1, aph = (it >> 1) & 1;
                 if (!mbar_wait(bar_acc_empty(buf), aph ^ 1, &abort_flag, &g_fg_error, 11)) break;
                 tc_fence_after();
@@ -214,25 +279,25 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
                     const uint32_t s = n % NS, ph = (n / NS) & 1;
                     if (!mbar_wait(bar_full(s), ph, &abort_flag, &g_fg_error, 12)) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(ring + (size_t)s * STAGE), sb = sa + A_BYTES;
+                    const uint32_t sa = smem_u32(ring + (size_t)s * S::STAGE), sb = sa + S::A_BYTES;
                     const uint64_t da = A_MN ? desc_mn_sw128(sa) : desc_sw128(sa), db = B_MN ? desc_mn_sw128(sb) : desc_sw128(sb);
 #pragma unroll
                     for (int j = 0; j < FG_BK / 16; ++j)  // 16 k further: 32 bytes inside the swizzled row, or two groups of 8 k (2048 bytes)
-                        tc_mma_f16(d, da + j * (A_MN ? 128 : 2), db + j * (B_MN ? 128 : 2), idesc, (kb | j) != 0);
-                    tc_commit(bar_empty(s));
+                        tc_mma_f16<CG>(d, da + j * (A_MN ? 128 : 2), db + j * (B_MN ? 128 : 2), idesc, (kb | j) != 0);
+                    tc_commit_pair<CG>(bar_empty(s));
                 }
-                tc_commit(bar_acc_full(buf));
+                tc_commit_pair<CG>(bar_acc_full(buf));
             }
         }
     } else if (warp >= 4) {
         const int q = warp & 3, half = warp >= 8 ? 1 : 0;
         uint32_t it = 0;
-        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++it) {
+        for (int i = first; i < tiles; i += step, ++it) {
             const Tile t = tile_at(i, P.m_tiles, P.n_tiles);
             const uint32_t buf = it & 1, aph = (it >> 1) & 1;
             if (!mbar_wait(bar_acc_full(buf), aph, &abort_flag, &g_fg_error, 21)) break;
             tc_fence_after();
-            const long long row = (long long)t.m * FG_BM + q * 32 + lane;
+            const long long row = (long long)(t.m * CG + (int)rank) * FG_BM + q * 32 + lane;
             const uint32_t t0 = tmem + ((uint32_t)(q * 32) << 16) + buf * BN;
             if (g.dual) {
                 for (int c = half * (BN / 4); c < (half + 1) * (BN / 4); c += 16) {
@@ -254,14 +319,22 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_acc_empty(buf));
+            if (lane == 0) {
+                if constexpr (CG == 2) mbar_arrive_cluster(map_rank(bar_acc_empty(buf), 0));
+                else mbar_arrive(bar_acc_empty(buf));
+            }
         }
     }
     tc_fence_before();
-    __syncthreads();
+    __syncwarp();
+    if constexpr (CG == 2) {
+        cluster_sync();  // neither CTA leaves while the other may still signal its barriers or read its shared memory
+    } else {
+        __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc_all<CG>(tmem);
     }
 }
 
@@ -280,21 +353,20 @@ static int fg_tmap(CUtensorMap* tm, const FgOperand& o, int is_f16, long long ro
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-template <typename T, int BN, bool A_MN, bool B_MN>
+template <typename T, int CG, int BN, bool A_MN, bool B_MN>
 static int fg_run(FgParams& P, cudaStream_t stream) {
-    constexpr uint32_t STAGE = (FG_BM + BN) * FG_BK * 2;
-    constexpr int NS = BN == 256 ? 4 : 6;
+    using S = FgShape<CG, BN>;
     const FgArgs& g = P.g;
-    P.m_tiles = (g.M + FG_BM - 1) / FG_BM;
+    P.m_tiles = (g.M + CG * FG_BM - 1) / (CG * FG_BM);
     P.n_tiles = g.dual ? (g.inter + BN / 2 - 1) / (BN / 2) : (g.N + BN - 1) / BN;
     P.k_blocks = (g.K + FG_BK - 1) / FG_BK;
-    if ((long long)P.m_tiles * P.n_tiles > 0x7FFFFFFFll) return ERR_TOO_LARGE;
+    if ((long long)P.m_tiles * P.n_tiles > 0x3FFFFFFFll) return ERR_TOO_LARGE;
     alignas(64) CUtensorMap ta, tb;
     int rc = fg_tmap(&ta, g.a, g.is_f16, g.M, g.K, FG_BM);
     if (!rc) rc = fg_tmap(&tb, g.b, g.is_f16, g.N, g.K, BN / 2);
     if (rc) return rc;
-    const size_t smem = (size_t)NS * STAGE + 1024;
-    auto kernel = fg_gemm_kernel<T, BN, A_MN, B_MN>;
+    const size_t smem = (size_t)S::NS * S::STAGE + 1024;
+    auto kernel = fg_gemm_kernel<T, CG, BN, A_MN, B_MN>;
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -303,14 +375,33 @@ static int fg_run(FgParams& P, cudaStream_t stream) {
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    const int tiles = P.m_tiles * P.n_tiles, sms = sm_count();
-    return (int)launch_pdl(kernel, dim3(tiles < sms ? tiles : sms), dim3(FG_THREADS), smem, stream, P, ta, tb);
+    const int tiles = P.m_tiles * P.n_tiles, groups = sm_count() / CG;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((tiles < groups ? tiles : groups) * CG);
+    cfg.blockDim = dim3(FG_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CG == 2 ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, P, ta, tb);
+}
+
+template <typename T, int CG, int BN>
+static int fg_layouts(FgParams& P, cudaStream_t stream) {
+    if (P.g.a.mn_major) return P.g.b.mn_major ? fg_run<T, CG, BN, true, true>(P, stream) : ERR_UNSUPPORTED;
+    return P.g.b.mn_major ? fg_run<T, CG, BN, false, true>(P, stream) : fg_run<T, CG, BN, false, false>(P, stream);
 }
 
 template <typename T>
 static int fg_dispatch(FgParams& P, cudaStream_t stream) {
-    if (P.g.a.mn_major) return P.g.b.mn_major ? fg_run<T, 128, true, true>(P, stream) : ERR_UNSUPPORTED;
-    return P.g.b.mn_major ? fg_run<T, 128, false, true>(P, stream) : fg_run<T, 128, false, false>(P, stream);
+    if (P.g.M <= FG_BM) return fg_layouts<T, 1, 128>(P, stream);
+    return fg_layouts<T, 2, 256>(P, stream);
 }
 
 int fg_launch(const FgArgs& a, cudaStream_t stream) {
