@@ -20,20 +20,24 @@ namespace b200 {
 __device__ int g_fg_error = 0;
 
 constexpr int FG_THREADS = 384;
-constexpr int FG_BM = 128, FG_BK = 64;  // rows of A per CTA, depth of a k block
+constexpr int FG_BM = 128, FG_BK = 64;  // rows of A per CTA, depth of a k block (a 128-byte row of 16-bit values)
 constexpr int FG_GROUP_M = 8;           // row tiles that are walked together down the columns: their A tiles stay in L2 while B passes once
-constexpr int FG_SMEM = 192 * 1024;     // ring of stages
+constexpr int FG_SMEM = 224 * 1024;     // ring of stages
 
+// A stage holds two k blocks: a turn of the producer's loop costs it about 240 clocks plus 48 per copy whatever the copies' size (measured with
+// copies alone), a 256 x 256 pair tile is done with a k block in 512.
 template <int CG, int BN>
 struct FgShape {
-    static constexpr uint32_t A_BYTES = FG_BM * FG_BK * 2, B_ROWS = BN / CG, B_BYTES = B_ROWS * FG_BK * 2, STAGE = A_BYTES + B_BYTES;
+    static constexpr uint32_t A_HALF = FG_BM * FG_BK * 2, B_ROWS = BN / CG, B_HALF = B_ROWS * FG_BK * 2, A_BYTES = 2 * A_HALF, B_BYTES = 2 * B_HALF, STAGE = A_BYTES + B_BYTES;
     static constexpr int NS = FG_SMEM / STAGE;
 };
 
 struct FgParams {
     FgArgs g;
     int m_tiles, n_tiles, k_blocks;
-    int vec_out, vec_res, vec_z, vec_bias;  // rows allow 16-byte accesses
+    int split;                              // CTAs (pairs) of a cluster that share the k blocks of one tile; 1: persistent CTAs
+    int vec_out, vec_res, vec_z, vec_bias;  // widest access that the rows allow: 2 = 32 bytes, 1 = 16 bytes, 0 = single values
+    int turned;                             // some row allows single values only: epilogue_turned
 };
 
 template <int CG>
@@ -49,9 +53,9 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t adesc, uint64_t 
 }
 // the MMAs issued so far, when done, arrive on this barrier (CG = 2: on the barrier at the same place in both CTAs of the pair)
 template <int CG>
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint32_t lead) {
     if constexpr (CG == 2)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)(3u << lead)) : "memory");
     else
         tc_commit(bar);
 }
@@ -94,16 +98,23 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
                  : "memory");
 }
 
-// MN-major operand tile with the 128-byte swizzle: boxes of 64 rows-of-the-operand x 64 k, [box][k][64]; 8 k are 1024 bytes apart (stride
+// MN-major operand tile with the 128-byte swizzle: boxes of 64 rows-of-the-operand x 128 k, [box][k][64]; 8 k are 1024 bytes apart (stride
 // offset), the next 64 operand rows one box further (leading offset).
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
 // instruction descriptor of kind::f16: fp32 accumulators, both operands of one 16-bit type, M = 128
 __device__ __forceinline__ uint32_t f16_idesc(int is_f16, int a_mn, int b_mn, int m, int n) {
     const uint32_t t = is_f16 ? 0u : 1u;
     return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+struct FgPick { int cg, bn, split; };
+
+// a wait whose phase is usually complete already: no look at the abort flag on that path
+__device__ __forceinline__ bool fg_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
+    return mbar_test(bar, parity) || mbar_wait(bar, parity, abort_flag, &g_fg_error, where);
 }
 
 struct Tile { int m, n; };
@@ -113,9 +124,29 @@ __device__ __forceinline__ Tile tile_at(int i, int m_tiles, int n_tiles) {
     return {first + r % gm, r / gm};
 }
 
+__device__ __forceinline__ void ldg32(const void* p, uint32_t (&a)[8]) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void stg32(void* p, const uint32_t (&a)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7])
+                 : "memory");
+}
+// 16 consecutive values of a row, of which the first n exist; a thread's row is one 32-byte sector wide here, so that the 32 rows of a warp
+// cost no partial sectors
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, bool vec, int n, float (&v)[16]) {
-    if (vec && n >= 16) {
+__device__ __forceinline__ void load16(const T* p, int vec, int n, float (&v)[16]) {
+    if (vec == 2 && n >= 16) {
+        uint32_t u[8];
+        ldg32(p, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = unpack2<T>(u[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    } else if (vec && n >= 16) {
         load8<T>(p, *reinterpret_cast<float(*)[8]>(&v[0]));
         load8<T>(p + 8, *reinterpret_cast<float(*)[8]>(&v[8]));
     } else {
@@ -124,8 +155,22 @@ __device__ __forceinline__ void load16(const T* p, bool vec, int n, float (&v)[1
     }
 }
 template <typename T>
-__device__ __forceinline__ void store16(T* p, bool vec, int n, const float (&v)[16]) {
-    if (vec && n >= 16) {
+__device__ __forceinline__ void store16(T* p, int vec, int n, const float (&v)[16]) {
+    if (vec == 2 && n >= 16) {
+        uint32_t u[8];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(v[8 * h + i]);
+                stg32(p + 8 * h, u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+            stg32(p, u);
+        }
+    } else if (vec && n >= 16) {
         store8<T>(p, *reinterpret_cast<const float(*)[8]>(&v[0]));
         store8<T>(p + 8, *reinterpret_cast<const float(*)[8]>(&v[8]));
     } else {
@@ -188,7 +233,52 @@ __device__ __forceinline__ void epilogue16_dual(const FgParams& P, long long row
     store16<T>(reinterpret_cast<T*>(g.out) + row * g.out_ld + col, P.vec_out, n, a);
 }
 
-template <typename T, int CG, int BN, bool A_MN, bool B_MN>
+// Rows that do not start on 16 bytes (an odd width, an odd offset): a thread per row would store single values, 32 rows apart.  The warp turns its
+// 32 rows x 32 accumulator columns around in shared memory and works on 32 (dual: 16) consecutive columns of a row at a time instead.
+constexpr int FG_TURN_LD = 33;
+constexpr int FG_TURN_BYTES = 8 * 32 * FG_TURN_LD * 4;
+template <typename T>
+__device__ __forceinline__ void epilogue_turned(const FgParams& P, float* buf, int lane, long long row0, int col0, const uint32_t (&a)[16], const uint32_t (&b)[16], int cols) {
+    const FgArgs& g = P.g;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        buf[lane * FG_TURN_LD + i] = __uint_as_float(a[i]);
+        buf[lane * FG_TURN_LD + 16 + i] = __uint_as_float(b[i]);
+    }
+    __syncwarp();
+    if (g.dual) {
+        const int col = col0 + (lane & 15);
+        for (int r = lane >> 4; r < 32; r += 2) {
+            const long long row = row0 + r;
+            if (row >= g.M || col >= g.inter) continue;
+            float z = buf[r * FG_TURN_LD + (lane & 15)], u = buf[r * FG_TURN_LD + 16 + (lane & 15)];
+            if (g.z_out) {
+                g.z_out[row * g.z_ld + col] = z;
+                g.z_out[row * g.z_ld + g.inter + col] = u;
+            }
+            if (g.limit > 0.f) {
+                z = z > g.limit ? g.limit : z;
+                u = u > g.limit ? g.limit : (u < -g.limit ? -g.limit : u);
+            }
+            reinterpret_cast<T*>(g.out)[row * g.out_ld + col] = from_f32<T>(act_fwd(g.act, z) * u);
+        }
+    } else {
+        const int col = col0 + lane;
+        if (lane >= cols || col >= g.N) return;
+        const float bias = g.bias ? to_f32(reinterpret_cast<const T*>(g.bias)[col]) : 0.f;
+        for (int r = 0; r < 32 && row0 + r < g.M; ++r) {
+            const long long row = row0 + r;
+            float z = buf[r * FG_TURN_LD + lane] + bias;
+            if (g.z_out) g.z_out[row * g.z_ld + col] = z;
+            z = act_fwd(g.act, z);
+            if (g.res) z += to_f32(reinterpret_cast<const T*>(g.res)[row * g.res_ld + col]);
+            reinterpret_cast<T*>(g.out)[row * g.out_ld + col] = from_f32<T>(z);
+        }
+    }
+}
+
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool SPLIT>
 __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P, const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b) {
     using S = FgShape<CG, BN>;
     constexpr int NS = S::NS;
@@ -197,7 +287,9 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
     __shared__ uint32_t tmem_base_sh;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = CG == 2 ? cluster_rank() : 0;  // the first CTA of a pair issues the MMAs; full[] and acc_empty[] are used there
+    const uint32_t crank = CG == 2 || SPLIT ? cluster_rank() : 0;
+    const uint32_t rank = crank & (CG - 1), lead = crank - rank;  // the first CTA of a pair issues the MMAs; full[] and acc_empty[] are used there
+    const int slice = SPLIT ? (int)crank / CG : 0, split = SPLIT ? P.split : 1;
     uint8_t* ring = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     auto bar_full = [&](int s) { return smem_u32(&bars[s]); };
     auto bar_empty = [&](int s) { return smem_u32(&bars[NS + s]); };
@@ -219,74 +311,90 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
     pdl_wait();
     pdl_launch_dependents();
     const FgArgs& g = P.g;
-    const int tiles = P.m_tiles * P.n_tiles, first = blockIdx.x / CG, step = gridDim.x / CG;
+    const int tiles = P.m_tiles * P.n_tiles, first = blockIdx.x / (CG * split), step = gridDim.x / (CG * split);
+    const int n_st = (P.k_blocks + 1) / 2;  // stages of a tile; this slice's: [st_lo, st_hi)
+    const int st_lo = SPLIT ? slice * n_st / split : 0, st_hi = SPLIT ? (slice + 1) * n_st / split : n_st;
+    float* turn = reinterpret_cast<float*>(ring + NS * S::STAGE) + (warp & 7) * 32 * FG_TURN_LD;
+    const uint32_t ring0 = smem_u32(ring), full0 = bar_full(0), empty0 = bar_empty(0);
 
     if (warp == 0) {
         if (lane == 0) {
             tma_prefetch_desc(&tm_a);
             tma_prefetch_desc(&tm_b);
-            uint32_t n = 0;
+            const uint32_t pair_full0 = CG == 2 ? map_rank(full0, lead) : full0;
+            uint32_t s = 0, ph = 1, n = 0;
             for (int i = first; i < tiles && !abort_flag; i += step) {
                 const Tile t = tile_at(i, P.m_tiles, P.n_tiles);
                 const int m0 = (t.m * CG + (int)rank) * FG_BM;
                 // the two halves of the B tile: consecutive rows, or gate rows and up rows; a CTA of a pair loads one of them
                 const int h0 = g.dual ? t.n * (BN / 2) : t.n * BN, h1 = g.dual ? g.inter + h0 : h0 + BN / 2;
                 const int n0 = rank ? h1 : h0;
-                for (int kb = 0; kb < P.k_blocks; ++kb, ++n) {
-                    const uint32_t s = n % NS, ph = (n / NS) & 1;
-                    if (!mbar_wait(bar_empty(s), ph ^ 1, &abort_flag, &g_fg_error, 1)) break;
-                    const uint32_t da = smem_u32(ring + (size_t)s * S::STAGE), db = da + S::A_BYTES;
-                    const int k0 = kb * FG_BK;
-                    if (rank == 0) mbar_expect_tx(bar_full(s), CG * S::STAGE);
-                    const uint32_t bar = CG == 2 ? map_rank(bar_full(s), 0) : bar_full(s);
+                for (int st = st_lo; st < st_hi; ++st, ++n) {
+                    if (!fg_wait(empty0 + 8 * s, ph, &abort_flag, 1)) break;
+                    const uint32_t da = ring0 + s * S::STAGE, db = da + S::A_BYTES, bar = pair_full0 + 8 * s;
+                    const int k0 = st * 2 * FG_BK;
+                    const bool two = 2 * st + 1 < P.k_blocks;  // the last stage may hold one k block
+                    if (rank == 0)
+                        mbar_expect_tx(full0 + 8 * s, CG * ((A_MN || two ? S::A_BYTES : S::A_HALF) + (B_MN || two ? S::B_BYTES : S::B_HALF)));
                     auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
                         if constexpr (CG == 2) tma_load_2d_pair(dst, tm, x, y, bar);
                         else tma_load_2d(dst, tm, x, y, bar);
                     };
                     if constexpr (A_MN) {
 #pragma unroll
-                        for (int q = 0; q < FG_BM / 64; ++q) load(da + q * 8192, &tm_a, m0 + q * 64, k0);
+                        for (int q = 0; q < FG_BM / 64; ++q) load(da + q * 16384, &tm_a, m0 + q * 64, k0);
                     } else {
                         load(da, &tm_a, k0, m0);
+                        if (two) load(da + S::A_HALF, &tm_a, k0 + FG_BK, m0);
                     }
                     if constexpr (B_MN) {
 #pragma unroll
-                        for (int q = 0; q < (int)S::B_ROWS / 64; ++q) load(db + q * 8192, &tm_b, n0 + q * 64, k0);
+                        for (int q = 0; q < (int)S::B_ROWS / 64; ++q) load(db + q * 16384, &tm_b, n0 + q * 64, k0);
                     } else {
                         load(db, &tm_b, k0, n0);
-                        if constexpr (CG == 1) load(db + S::B_BYTES / 2, &tm_b, k0, h1);
+                        if constexpr (CG == 1) load(db + S::B_HALF / 2, &tm_b, k0, h1);
+                        if (two) {
+                            load(db + S::B_HALF, &tm_b, k0 + FG_BK, n0);
+                            if constexpr (CG == 1) load(db + S::B_HALF + S::B_HALF / 2, &tm_b, k0 + FG_BK, h1);
+                        }
                     }
+                    if (++s == NS) { s = 0; ph ^= 1; }
                 }
             }
             // every load issued above must have landed before the CTA may exit (the second CTA of a pair is kept by the cluster barrier below)
             for (int k = 0; rank == 0 && k < NS && k < (int)n; ++k) {
-                const uint32_t m = n - 1 - k, s = m % NS, ph = (m / NS) & 1;
+                const uint32_t m = n - 1 - k, s2 = m % NS, ph2 = (m / NS) & 1;
                 const unsigned long long t0 = global_timer_ns();
-                while (!mbar_test(bar_full(s), ph))
+                while (!mbar_test(bar_full(s2), ph2))
                     if (global_timer_ns() - t0 > WAIT_LIMIT_NS) { atomicCAS(&g_fg_error, 0, 2); break; }
             }
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             const uint32_t idesc = f16_idesc(g.is_f16, A_MN, B_MN, FG_BM * CG, BN);
-            uint32_t n = 0, it = 0;
+            const uint64_t desc_a0 = A_MN ? desc_mn_sw128(ring0) : desc_sw128(ring0);
+            const uint64_t desc_b0 = B_MN ? desc_mn_sw128(ring0 + S::A_BYTES) : desc_sw128(ring0 + S::A_BYTES);
+            uint32_t s = 0, ph = 0, it = 0;
             for (int i = first; i < tiles && !abort_flag; i += step, ++it) {
                 const uint32_t buf = it & 1, aph = (it >> 1) & 1;
-                if (!mbar_wait(bar_acc_empty(buf), aph ^ 1, &abort_flag, &g_fg_error, 11)) break;
+                if (!fg_wait(bar_acc_empty(buf), aph ^ 1, &abort_flag, 11)) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * BN;
-                for (int kb = 0; kb < P.k_blocks; ++kb, ++n) {
-                    const uint32_t s = n % NS, ph = (n / NS) & 1;
-                    if (!mbar_wait(bar_full(s), ph, &abort_flag, &g_fg_error, 12)) break;
+                for (int st = st_lo; st < st_hi; ++st) {
+                    if (!fg_wait(full0 + 8 * s, ph, &abort_flag, 12)) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(ring + (size_t)s * S::STAGE), sb = sa + S::A_BYTES;
-                    const uint64_t da = A_MN ? desc_mn_sw128(sa) : desc_sw128(sa), db = B_MN ? desc_mn_sw128(sb) : desc_sw128(sb);
+                    const uint64_t da = desc_a0 + s * (S::STAGE >> 4), db = desc_b0 + s * (S::STAGE >> 4);
 #pragma unroll
-                    for (int j = 0; j < FG_BK / 16; ++j)  // 16 k further: 32 bytes inside the swizzled row, or two groups of 8 k (2048 bytes)
-                        tc_mma_f16<CG>(d, da + j * (A_MN ? 128 : 2), db + j * (B_MN ? 128 : 2), idesc, (kb | j) != 0);
-                    tc_commit_pair<CG>(bar_empty(s));
+                    for (int j = 0; j < 2 * FG_BK / 16; ++j) {
+                        if (j == FG_BK / 16 && 2 * st + 1 >= P.k_blocks) break;
+                        // 16 k further: 32 bytes inside the swizzled row (then the second k block), or two groups of 8 k (2048 bytes)
+                        const uint32_t oa = A_MN ? j * 128 : (j & 3) * 2 + (j >> 2) * (S::A_HALF >> 4), ob = B_MN ? j * 128 : (j & 3) * 2 + (j >> 2) * (S::B_HALF >> 4);
+                        tc_mma_f16<CG>(d, da + oa, db + ob, idesc, st != st_lo || j != 0);
+                    }
+                    tc_commit_pair<CG>(empty0 + 8 * s, lead);
+                    if (++s == NS) { s = 0; ph ^= 1; }
                 }
-                tc_commit_pair<CG>(bar_acc_full(buf));
+                tc_commit_pair<CG>(bar_acc_full(buf), lead);
             }
         }
     } else if (warp >= 4) {
@@ -295,8 +403,9 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
         for (int i = first; i < tiles; i += step, ++it) {
             const Tile t = tile_at(i, P.m_tiles, P.n_tiles);
             const uint32_t buf = it & 1, aph = (it >> 1) & 1;
-            if (!mbar_wait(bar_acc_full(buf), aph, &abort_flag, &g_fg_error, 21)) break;
+            if (!fg_wait(bar_acc_full(buf), aph, &abort_flag, 21)) break;
             tc_fence_after();
+            if constexpr (SPLIT) break;  // the parts of the tile are added below
             const long long row = (long long)(t.m * CG + (int)rank) * FG_BM + q * 32 + lane;
             const uint32_t t0 = tmem + ((uint32_t)(q * 32) << 16) + buf * BN;
             if (g.dual) {
@@ -306,32 +415,111 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
                     tc_ld16(t0 + BN / 2 + c, b);
                     tc_wait_ld();
                     const int col = t.n * (BN / 2) + c;
-                    if (row < g.M && col < g.inter) epilogue16_dual<T>(P, row, col, a, b);
+                    if (P.turned) epilogue_turned<T>(P, turn, lane, row - lane, col, a, b, 16);
+                    else if (row < g.M && col < g.inter) epilogue16_dual<T>(P, row, col, a, b);
                 }
             } else {
-                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 16) {
-                    uint32_t a[16];
+                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+                    uint32_t a[16], b[16];
                     tc_ld16(t0 + c, a);
+                    tc_ld16(t0 + c + 16, b);
                     tc_wait_ld();
                     const int col = t.n * BN + c;
-                    if (row < g.M && col < g.N) epilogue16<T>(P, row, col, a);
+                    if (P.turned) {
+                        epilogue_turned<T>(P, turn, lane, row - lane, col, a, b, 32);
+                    } else if (row < g.M) {
+                        if (col < g.N) epilogue16<T>(P, row, col, a);
+                        if (col + 16 < g.N) epilogue16<T>(P, row, col + 16, b);
+                    }
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (CG == 2) mbar_arrive_cluster(map_rank(bar_acc_empty(buf), 0));
+                if constexpr (CG == 2) mbar_arrive_cluster(map_rank(bar_acc_empty(buf), lead));
                 else mbar_arrive(bar_acc_empty(buf));
+            }
+        }
+    }
+    if constexpr (SPLIT) {
+        // One tile per cluster, its k blocks shared by the `split` CTAs (pairs).  Each of them finishes BN / split of the columns: it gets the
+        // others' accumulators of those columns in its shared memory (the ring is free by now), [slice][4 columns][row], and adds the parts
+        // in slice order.
+        const int W = BN / split, W2 = W / 2, nj = W / 16, n2 = g.dual ? nj / 2 : 0;
+        const int q = warp & 3, half = warp >= 8 ? 1 : 0, r = q * 32 + lane;
+        const uint32_t t0 = tmem + ((uint32_t)(q * 32) << 16);
+        auto column = [&](int owner, int j) { return g.dual ? (j < n2 ? owner * W2 + 16 * j : BN / 2 + owner * W2 + 16 * (j - n2)) : owner * W + 16 * j; };
+        __syncwarp();
+        cluster_sync();  // every CTA's MMAs have read their stages
+        tc_fence_after();
+        if (warp >= 4) {
+            for (int o = 0; o < split; ++o) {
+                if (o == slice) continue;
+                const uint32_t dst = map_rank(smem_u32(ring), (uint32_t)(o * CG) + rank) + (uint32_t)(slice * (W / 4) * FG_BM + r) * 16u;
+                for (int j = half; j < nj; j += 2) {
+                    uint32_t a[16];
+                    tc_ld16(t0 + column(o, j), a);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)((4 * j + i) * FG_BM) * 16u), "r"(a[4 * i]), "r"(a[4 * i + 1]),
+                                     "r"(a[4 * i + 2]), "r"(a[4 * i + 3])
+                                     : "memory");
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 4) {
+            const Tile t = tile_at(first, P.m_tiles, P.n_tiles);
+            const long long row = (long long)(t.m * CG + (int)rank) * FG_BM + r;
+            auto sum16 = [&](int j, uint32_t (&out)[16]) {
+                uint32_t a[16];
+                tc_ld16(t0 + column(slice, j), a);
+                tc_wait_ld();
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = 0.f;
+                for (int sl = 0; sl < split; ++sl) {
+                    if (sl == slice) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] += __uint_as_float(a[i]);
+                    } else {
+                        const float4* src = reinterpret_cast<const float4*>(ring) + (sl * (W / 4) + 4 * j) * FG_BM + r;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 f = src[i * FG_BM];
+                            v[4 * i] += f.x; v[4 * i + 1] += f.y; v[4 * i + 2] += f.z; v[4 * i + 3] += f.w;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[i] = __float_as_uint(v[i]);
+            };
+            if (g.dual) {
+                for (int j = half; j < n2; j += 2) {
+                    uint32_t a[16], b[16];
+                    sum16(j, a);
+                    sum16(n2 + j, b);
+                    const int col = t.n * (BN / 2) + slice * W2 + 16 * j;
+                    if (P.turned) epilogue_turned<T>(P, turn, lane, row - lane, col, a, b, 16);
+                    else if (row < g.M && col < g.inter) epilogue16_dual<T>(P, row, col, a, b);
+                }
+            } else {
+                for (int j = half; j < nj; j += 2) {
+                    uint32_t a[16];
+                    sum16(j, a);
+                    const int col = t.n * BN + slice * W + 16 * j;
+                    if (P.turned) epilogue_turned<T>(P, turn, lane, row - lane, col, a, a, 16);
+                    else if (row < g.M && col < g.N) epilogue16<T>(P, row, col, a);
+                }
             }
         }
     }
     tc_fence_before();
     __syncwarp();
-    if constexpr (CG == 2) {
-        cluster_sync();  // neither CTA leaves while the other may still signal its barriers or read its shared memory
-    } else {
-        __syncthreads();
-    }
+    if constexpr (CG == 2 || SPLIT) cluster_sync();  // no CTA leaves while another may still signal its barriers or read its shared memory
+    else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc_all<CG>(tmem);
@@ -346,38 +534,39 @@ static int fg_tmap(CUtensorMap* tm, const FgOperand& o, int is_f16, long long ro
     if (!fn) return (int)cudaErrorNotSupported;
     cuuint64_t dims[2] = {(cuuint64_t)(o.mn_major ? rows : k), (cuuint64_t)(o.mn_major ? k : rows)};
     cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
-    cuuint32_t box[2] = {64, o.mn_major ? 64u : box_rows};
+    cuuint32_t box[2] = {64, o.mn_major ? 2u * FG_BK : box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(tm, is_f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(o.base), dims, strides, box, estr,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-template <typename T, int CG, int BN, bool A_MN, bool B_MN>
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool SPLIT>
 static int fg_run(FgParams& P, cudaStream_t stream) {
     using S = FgShape<CG, BN>;
     const FgArgs& g = P.g;
     P.m_tiles = (g.M + CG * FG_BM - 1) / (CG * FG_BM);
     P.n_tiles = g.dual ? (g.inter + BN / 2 - 1) / (BN / 2) : (g.N + BN - 1) / BN;
     P.k_blocks = (g.K + FG_BK - 1) / FG_BK;
-    if ((long long)P.m_tiles * P.n_tiles > 0x3FFFFFFFll) return ERR_TOO_LARGE;
+    if ((long long)P.m_tiles * P.n_tiles > 0x0FFFFFFFll) return ERR_TOO_LARGE;
     alignas(64) CUtensorMap ta, tb;
     int rc = fg_tmap(&ta, g.a, g.is_f16, g.M, g.K, FG_BM);
     if (!rc) rc = fg_tmap(&tb, g.b, g.is_f16, g.N, g.K, BN / 2);
     if (rc) return rc;
-    const size_t smem = (size_t)S::NS * S::STAGE + 1024;
-    auto kernel = fg_gemm_kernel<T, CG, BN, A_MN, B_MN>;
+    const size_t smem = (size_t)S::NS * S::STAGE + 1024 + (P.turned ? FG_TURN_BYTES : 0);
+    constexpr int smem_max = S::NS * S::STAGE + 1024 + (BN == 192 ? 0 : FG_TURN_BYTES);
+    auto kernel = fg_gemm_kernel<T, CG, BN, A_MN, B_MN, SPLIT>;
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max);
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    const int tiles = P.m_tiles * P.n_tiles, groups = sm_count() / CG;
+    const int tiles = P.m_tiles * P.n_tiles, groups = sm_count() / CG, cluster = CG * P.split;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((tiles < groups ? tiles : groups) * CG);
+    cfg.gridDim = dim3(SPLIT ? tiles * cluster : (tiles < groups ? tiles : groups) * CG);
     cfg.blockDim = dim3(FG_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -385,23 +574,57 @@ static int fg_run(FgParams& P, cudaStream_t stream) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = CG;
+    attr[1].val.clusterDim.x = cluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = CG == 2 ? 2 : 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, kernel, P, ta, tb);
 }
 
-template <typename T, int CG, int BN>
+template <typename T, int CG, int BN, bool SPLIT>
 static int fg_layouts(FgParams& P, cudaStream_t stream) {
-    if (P.g.a.mn_major) return P.g.b.mn_major ? fg_run<T, CG, BN, true, true>(P, stream) : ERR_UNSUPPORTED;
-    return P.g.b.mn_major ? fg_run<T, CG, BN, false, true>(P, stream) : fg_run<T, CG, BN, false, false>(P, stream);
+    if constexpr (BN == 192) {  // MN-major boxes are 64 rows wide: a pair's 96 rows of B are no multiple of that
+        return P.g.b.mn_major || P.g.a.mn_major ? ERR_UNSUPPORTED : fg_run<T, CG, BN, false, false, SPLIT>(P, stream);
+    } else {
+        if (P.g.a.mn_major) return P.g.b.mn_major ? fg_run<T, CG, BN, true, true, SPLIT>(P, stream) : ERR_UNSUPPORTED;
+        return P.g.b.mn_major ? fg_run<T, CG, BN, false, true, SPLIT>(P, stream) : fg_run<T, CG, BN, false, false, SPLIT>(P, stream);
+    }
+}
+
+// Which tile, and how many ways its k is split.  Each choice's time is estimated as (turns of the busiest CTA) x (stages of a tile) x (time of a
+// stage) + (start, end and last epilogue), the constants in us from measurements over 25 shapes between 64 x 4096 x 2048 and 8192 x 8192 x
+// 8192; e.g. measured 64 x 4096 x 4096: 1/128/4 13.9, 1/128/1 20.9, 2/256/1 25.7; 512 x 4096 x 4096: 2/256/2 21.3, 1/128/1 22.0, 1/128/4 47.5;
+// 1500 x 4096 x 4096: 2/192/1 41.9, 2/256/1 48.0, 1/128/1 55.9; 4096 x 12288 x 4096: 2/256/1 275, 2/192/1 290, 1/128/1 384.
+static FgPick fg_pick(const FgParams& P) {
+    const FgArgs& g = P.g;
+    static const struct { FgPick k; double stage, fixed; } choices[] = {
+        {{1, 128, 1}, .54, 4.0}, {{1, 128, 2}, .54, 7.5}, {{1, 128, 4}, .54, 8.5}, {{2, 128, 1}, .54, 4.5},  {{2, 128, 2}, .54, 8.0},
+        {{2, 192, 1}, .645, 5.5}, {{2, 256, 1}, .78, 6.5}, {{2, 256, 2}, .78, 10.0}};
+    const int st = (g.K + 2 * FG_BK - 1) / (2 * FG_BK), sms = sm_count();
+    FgPick best{2, 256, 1};
+    double best_t = 1e30;
+    for (const auto& c : choices) {
+        const FgPick& k = c.k;
+        if (k.split > st || (k.bn == 192 && (g.a.mn_major || g.b.mn_major || P.turned))) continue;
+        const int cols = g.dual ? k.bn / 2 : k.bn, width = g.dual ? g.inter : g.N;
+        const long long tiles = ((long long)g.M + k.cg * FG_BM - 1) / (k.cg * FG_BM) * ((width + cols - 1) / cols);
+        const int groups = sms / (k.cg * k.split);
+        const double turns = (double)((tiles + groups - 1) / groups);
+        // persistent CTAs pay the fixed part once, clusters that split a tile once per turn
+        const double t = k.split > 1 ? turns * ((st + k.split - 1) / k.split * c.stage + c.fixed) : turns * st * c.stage + c.fixed;
+        if (t < best_t) { best_t = t; best = k; }
+    }
+    return best;
 }
 
 template <typename T>
 static int fg_dispatch(FgParams& P, cudaStream_t stream) {
-    if (P.g.M <= FG_BM) return fg_layouts<T, 1, 128>(P, stream);
-    return fg_layouts<T, 2, 256>(P, stream);
+    const FgPick k = fg_pick(P);
+    P.split = k.split;
+    if (k.cg == 1) return k.split > 1 ? fg_layouts<T, 1, 128, true>(P, stream) : fg_layouts<T, 1, 128, false>(P, stream);
+    if (k.bn == 128) return k.split > 1 ? fg_layouts<T, 2, 128, true>(P, stream) : fg_layouts<T, 2, 128, false>(P, stream);
+    if (k.bn == 192) return fg_layouts<T, 2, 192, false>(P, stream);
+    return k.split > 1 ? fg_layouts<T, 2, 256, true>(P, stream) : fg_layouts<T, 2, 256, false>(P, stream);
 }
 
 int fg_launch(const FgArgs& a, cudaStream_t stream) {
@@ -413,11 +636,15 @@ int fg_launch(const FgArgs& a, cudaStream_t stream) {
     if (a.M <= FS_MAX_M && !a.a.mn_major && !a.b.mn_major) return fs_launch(a, stream);
     FgParams P{};
     P.g = a;
-    auto vec = [](const void* p, long long ld) { return p && !((uintptr_t)p & 15) && ld % 8 == 0; };
-    P.vec_out = vec(a.out, a.out_ld);
-    P.vec_res = vec(a.res, a.res_ld);
-    P.vec_z = vec(a.z_out, a.z_ld) && (!a.dual || a.inter % 8 == 0);
+    auto vec = [](const void* p, long long ld_bytes) {
+        const uintptr_t u = (uintptr_t)p | (uintptr_t)ld_bytes;
+        return u & 15 ? 0 : (u & 31 ? 1 : 2);
+    };
+    P.vec_out = vec(a.out, a.out_ld * 2);
+    P.vec_res = vec(a.res, a.res_ld * 2);
+    P.vec_z = vec(a.z_out, a.dual ? a.z_ld * 4 | a.inter * 4 : a.z_ld * 4);
     P.vec_bias = vec(a.bias, 0);
+    P.turned = !P.vec_out || (a.res && !P.vec_res) || (a.z_out && !P.vec_z);
     return a.is_f16 ? fg_dispatch<__half>(P, stream) : fg_dispatch<__nv_bfloat16>(P, stream);
 }
 
