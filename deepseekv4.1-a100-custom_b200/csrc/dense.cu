@@ -87,20 +87,23 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy
     store_vec<T, VEC>(dgu + r * dgu_ld + inter + c, u);
 }
 
-// rows of any width and address into rows that start on 16 bytes (dst_ld a multiple of 8): a tensor map needs that
-__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restrict__ src, long long src_ld, uint16_t* __restrict__ dst, long long dst_ld, long long rows,
-                                                         int cols) {
+// Rows of any width and address into rows that start on 16 bytes (dst_ld a multiple of 8): a tensor map needs that.  One or two matrices of
+// the same width in a launch.
+struct AlignRows { const uint16_t* src; long long src_ld; uint16_t* dst; long long rows; };
+__global__ void __launch_bounds__(256) align_rows_kernel(const AlignRows m0, const AlignRows m1, long long dst_ld, int cols) {
     pdl_wait();
     pdl_launch_dependents();
     const int per_row = (cols + 7) / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
-    if (r >= rows) return;
-    const int c = (int)(i - r * per_row) * 8;
-    const uint16_t* s = src + r * src_ld + c;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, ri = i / per_row;
+    if (ri >= m0.rows + m1.rows) return;
+    const bool second = ri >= m0.rows;
+    const long long r = second ? ri - m0.rows : ri;
+    const int c = (int)(i - ri * per_row) * 8;
+    const uint16_t* s = (second ? m1.src + r * m1.src_ld : m0.src + r * m0.src_ld) + c;
     uint32_t v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? s[k] : 0;  // the rest of the last 16 bytes: zeros
-    *reinterpret_cast<uint4*>(dst + r * dst_ld + c) = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    *reinterpret_cast<uint4*>((second ? m1.dst : m0.dst) + r * dst_ld + c) = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
 // e4m3 codes with one E8M0 scale per 32 k (row r's scales in row r >> row_shift of sf) -> bf16, exactly: 4 significant bits times a power of two
@@ -235,14 +238,16 @@ extern "C" int b200_gated_linear_bwd(const void* gy, long long gy_ld, const floa
                            : gated_bwd_run<__half>(gy, gy_ld, gu, gu_ld, act, limit, M, inter, dgu, dgu_ld, stream);
 }
 
-extern "C" int b200_align_rows(const void* src, long long src_ld, void* dst, long long dst_ld, long long rows, int cols, cudaStream_t stream) {
-    if (rows < 0 || cols <= 0 || src_ld < 0 || dst_ld < cols) return ERR_BAD_SHAPE;
-    if (rows == 0) return 0;
-    if (!src || !dst) return ERR_BAD_ARG;
-    if (((uintptr_t)src & 1) || !ok16(dst, dst_ld)) return ERR_BAD_ALIGN;
-    const long long blocks = (rows * ((cols + 7) / 8) + 255) / 256;
+extern "C" int b200_align_rows(const void* src, long long src_ld, void* dst, long long rows, const void* src2, long long src2_ld, void* dst2, long long rows2, int cols,
+                               long long dst_ld, cudaStream_t stream) {
+    if (rows < 0 || rows2 < 0 || cols <= 0 || src_ld < 0 || src2_ld < 0 || dst_ld < cols) return ERR_BAD_SHAPE;
+    if (rows + rows2 == 0) return 0;
+    if ((rows && (!src || !dst)) || (rows2 && (!src2 || !dst2))) return ERR_BAD_ARG;
+    if (((uintptr_t)src & 1) || ((uintptr_t)src2 & 1) || !ok16(dst, dst_ld) || !ok16(dst2, dst_ld)) return ERR_BAD_ALIGN;
+    const long long blocks = ((rows + rows2) * ((cols + 7) / 8) + 255) / 256;
     if (blocks > 0x7FFFFFFFll) return ERR_TOO_LARGE;
-    return (int)launch_pdl(align_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (const uint16_t*)src, src_ld, (uint16_t*)dst, dst_ld, rows, cols);
+    return (int)launch_pdl(align_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, AlignRows{(const uint16_t*)src, src_ld, (uint16_t*)dst, rows},
+                           AlignRows{(const uint16_t*)src2, src2_ld, (uint16_t*)dst2, rows2}, dst_ld, cols);
 }
 
 extern "C" size_t b200_linear_act_q8_workspace_bytes(int M, int N, int K) {

@@ -249,10 +249,13 @@ __device__ __forceinline__ void epilogue_turned(const FgParams& P, float* buf, i
     __syncwarp();
     if (g.dual) {
         const int col = col0 + (lane & 15);
-        for (int r = lane >> 4; r < 32; r += 2) {
+        if (col >= g.inter) return;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+            const int r = 2 * i + (lane >> 4);
             const long long row = row0 + r;
-            if (row >= g.M || col >= g.inter) continue;
             float z = buf[r * FG_TURN_LD + (lane & 15)], u = buf[r * FG_TURN_LD + 16 + (lane & 15)];
+            if (row >= g.M) continue;
             if (g.z_out) {
                 g.z_out[row * g.z_ld + col] = z;
                 g.z_out[row * g.z_ld + g.inter + col] = u;
@@ -267,13 +270,21 @@ __device__ __forceinline__ void epilogue_turned(const FgParams& P, float* buf, i
         const int col = col0 + lane;
         if (lane >= cols || col >= g.N) return;
         const float bias = g.bias ? to_f32(reinterpret_cast<const T*>(g.bias)[col]) : 0.f;
-        for (int r = 0; r < 32 && row0 + r < g.M; ++r) {
-            const long long row = row0 + r;
-            float z = buf[r * FG_TURN_LD + lane] + bias;
-            if (g.z_out) g.z_out[row * g.z_ld + col] = z;
-            z = act_fwd(g.act, z);
-            if (g.res) z += to_f32(reinterpret_cast<const T*>(g.res)[row * g.res_ld + col]);
-            reinterpret_cast<T*>(g.out)[row * g.out_ld + col] = from_f32<T>(z);
+        const T* res = reinterpret_cast<const T*>(g.res);
+        const int rows = g.M - row0 < 32 ? (int)(g.M - row0) : 32;
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+            float rv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rv[i] = res && r0 + i < rows ? to_f32(res[(row0 + r0 + i) * g.res_ld + col]) : 0.f;  // in flight together
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i;
+                if (r >= rows) break;
+                float z = buf[r * FG_TURN_LD + lane] + bias;
+                if (g.z_out) g.z_out[(row0 + r) * g.z_ld + col] = z;
+                z = act_fwd(g.act, z) + rv[i];
+                reinterpret_cast<T*>(g.out)[(row0 + r) * g.out_ld + col] = from_f32<T>(z);
+            }
         }
     }
 }

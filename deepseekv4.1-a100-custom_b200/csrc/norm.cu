@@ -71,8 +71,8 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(const NormArgs a, in
     __shared__ float red[32];
     pdl_wait();
     pdl_launch_dependents();
-    const int t = threadIdx.x & (tpr - 1);
-    const long long row = (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+    const int t = tpr == 32 ? threadIdx.x & 31 : threadIdx.x;  // several rows of 32 threads per block, or one of more
+    const long long row = tpr == 32 ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const bool live = row < a.rows;  // a dead row's threads still take part in the shuffles
     const T* x = reinterpret_cast<const T*>(a.x) + (live ? row : 0) * a.x_ld;
     const T* r = a.r ? reinterpret_cast<const T*>(a.r) + (live ? row : 0) * a.r_ld : nullptr;
@@ -146,7 +146,36 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(const NormArgs a, in
 
 // Backward.  With n = s rinv and h = gy w:  ds = rinv (h - n mean(h n)) + gs,  dw = sum over rows of gy n.
 // Blocks walk the rows with the grid's stride and keep their part of dw in registers; the parts are added in block order by
-// column_sum_kernel (no atomics: the same result from run to run).
+// column_sum_kernel (no atomics: the same result from run to run).  The next row's loads are issued before this row's reduction, so that the
+// memory works through the barriers.
+template <typename T, int VEC> struct RawVec { static constexpr int WORDS = sizeof(T) * VEC / 4; uint32_t u[WORDS]; };
+template <typename T> struct RawVec<T, 1> { T u; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_raw(const T* p, RawVec<T, VEC>& r) {
+    if constexpr (VEC == 1) r.u = *p;
+    else
+#pragma unroll
+        for (int i = 0; i < RawVec<T, VEC>::WORDS / 4; ++i) {
+            const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+            r.u[4 * i] = q.x; r.u[4 * i + 1] = q.y; r.u[4 * i + 2] = q.z; r.u[4 * i + 3] = q.w;
+        }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void value_of(const RawVec<T, VEC>& r, float (&v)[VEC]) {
+    if constexpr (VEC == 1) v[0] = to_f32(r.u);
+    else if constexpr (sizeof(T) == 4)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(r.u[i]);
+    else
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            const float2 f = unpack2<T>(r.u[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+}
+
 template <typename T, int VEC, int NV>
 __global__ void __launch_bounds__(VEC == 8 ? 512 : 1024) add_rms_norm_bwd_kernel(const NormArgs a, int tpr) {
     __shared__ float red[64];
@@ -158,29 +187,54 @@ __global__ void __launch_bounds__(VEC == 8 ? 512 : 1024) add_rms_norm_bwd_kernel
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    RawVec<T, VEC> rx[NV], rr[NV], rg[NV], rs[NV];
+    auto fetch = [&](long long row) {
         const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_ld;
         const T* r = a.r ? reinterpret_cast<const T*>(a.r) + row * a.r_ld : nullptr;
         const T* gy = reinterpret_cast<const T*>(a.gy) + row * a.dim;
         const T* gs = a.gs ? reinterpret_cast<const T*>(a.gs) + row * a.dim : nullptr;
-        float s[NV][VEC], g[NV][VEC];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (t + j * tpr) * VEC;
+            if (c < a.dim) {
+                load_raw<T, VEC>(x + c, rx[j]);
+                load_raw<T, VEC>(gy + c, rg[j]);
+                if (r) load_raw<T, VEC>(r + c, rr[j]);
+                if (gs) load_raw<T, VEC>(gs + c, rs[j]);
+            }
+        }
+    };
+    if (blockIdx.x < a.rows) fetch(blockIdx.x);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        float s[NV][VEC], g[NV][VEC], d[NV][VEC];
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (t + j * tpr) * VEC;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s[j][i] = g[j][i] = 0.f;
+            for (int i = 0; i < VEC; ++i) s[j][i] = g[j][i] = d[j][i] = 0.f;
             if (c < a.dim) {
-                load_vec<T, VEC>(x + c, s[j]);
-                load_vec<T, VEC>(gy + c, g[j]);
-                if (r) {
-                    float v[VEC];
-                    load_vec<T, VEC>(r + c, v);
+                float w[VEC], v[VEC];
+                load_weight<T, VEC>(a, c, w);
+                value_of<T, VEC>(rx[j], s[j]);
+                value_of<T, VEC>(rg[j], g[j]);
+                if (a.r) {
+                    value_of<T, VEC>(rr[j], v);
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) s[j][i] += v[i];
                 }
+                if (a.gs) value_of<T, VEC>(rs[j], d[j]);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    sum[0] += s[j][i] * s[j][i];
+                    sum[1] += g[j][i] * w[i] * s[j][i];
+                }
             }
         }
+        if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
+        row_sum<2>(sum, tpr, red);
+        const float rinv = rsqrtf(sum[0] / (float)a.dim + a.eps);
+        const float k = rinv * rinv * (sum[1] / (float)a.dim);  // n mean(h n) = s rinv * rinv mean(h s)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (t + j * tpr) * VEC;
@@ -189,32 +243,10 @@ __global__ void __launch_bounds__(VEC == 8 ? 512 : 1024) add_rms_norm_bwd_kernel
                 load_weight<T, VEC>(a, c, w);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    sum[0] += s[j][i] * s[j][i];
-                    sum[1] += g[j][i] * w[i] * s[j][i];
-                }
-            }
-        }
-        row_sum<2>(sum, tpr, red);
-        const float rinv = rsqrtf(sum[0] / (float)a.dim + a.eps);
-        const float k = rinv * rinv * (sum[1] / (float)a.dim);  // n mean(h n) = s rinv * rinv mean(h s)
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = (t + j * tpr) * VEC;
-            if (c < a.dim) {
-                float w[VEC], d[VEC];
-                load_weight<T, VEC>(a, c, w);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    d[i] = rinv * (g[j][i] * w[i] - s[j][i] * k);
+                    d[j][i] += rinv * (g[j][i] * w[i] - s[j][i] * k);
                     dw[j][i] += g[j][i] * (s[j][i] * rinv);
                 }
-                if (gs) {
-                    float v[VEC];
-                    load_vec<T, VEC>(gs + c, v);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) d[i] += v[i];
-                }
-                store_vec<T, VEC>(reinterpret_cast<T*>(a.ds) + row * a.dim + c, d);
+                store_vec<T, VEC>(reinterpret_cast<T*>(a.ds) + row * a.dim + c, d[j]);
             }
         }
     }
@@ -227,27 +259,29 @@ __global__ void __launch_bounds__(VEC == 8 ? 512 : 1024) add_rms_norm_bwd_kernel
     }
 }
 
-// out[c] = sum of part[p][c] over p, in a fixed order: 8 slices of the parts by the 8 rows of threads, then the slices
+// out[c] = sum of part[p][c] over p, in a fixed order: 32 slices of the parts by the 32 warps of a block, then the slices
 template <typename T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, int parts, int dim, T* __restrict__ out) {
-    __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, int parts, int dim, T* __restrict__ out) {
+    __shared__ float red[32][33];
     pdl_wait();
     pdl_launch_dependents();
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, sl = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float acc = 0.f;
-    if (c < dim)
-        for (int p = sl; p < parts; p += 8) acc += part[(long long)p * dim + c];
-    red[sl][threadIdx.x & 31] = acc;
+    if (c < dim) {
+#pragma unroll 8
+        for (int p = sl; p < parts; p += 32) acc += part[(long long)p * dim + c];
+    }
+    red[sl][lane] = acc;
     __syncthreads();
     if (sl == 0 && c < dim) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) acc += red[i][threadIdx.x & 31];
+        for (int i = 1; i < 32; ++i) acc += red[i][lane];
         out[c] = from_f32<T>(acc);
     }
 }
 
 int column_sum(const float* part, int parts, int dim, int dtype, void* out, cudaStream_t stream) {
-    const dim3 g((dim + 31) / 32), b(256);
+    const dim3 g((dim + 31) / 32), b(1024);
     if (dtype == F_FP32) return (int)launch_pdl(column_sum_kernel<float>, g, b, 0, stream, part, parts, dim, (float*)out);
     if (dtype == F_BF16) return (int)launch_pdl(column_sum_kernel<__nv_bfloat16>, g, b, 0, stream, part, parts, dim, (__nv_bfloat16*)out);
     return (int)launch_pdl(column_sum_kernel<__half>, g, b, 0, stream, part, parts, dim, (__half*)out);
@@ -258,12 +292,8 @@ int sm_count();
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// threads per row: the power of two (32 at least) with which a thread holds at most `nv` vectors
-static int threads_per_row(int dim, int vec, int nv) {
-    int tpr = 32;
-    while (tpr * vec * nv < dim) tpr *= 2;
-    return tpr;
-}
+// threads per row, whole warps, so that a thread holds at most `nv` vectors
+static int threads_per_row(int dim, int vec, int nv) { return (dim + vec * nv * 32 - 1) / (vec * nv * 32) * 32; }
 
 template <typename T, int VEC, int NV, bool QUANT>
 static int launch_fwd(const NormArgs& a, int tpr, cudaStream_t stream) {
@@ -276,8 +306,14 @@ static int launch_fwd(const NormArgs& a, int tpr, cudaStream_t stream) {
 template <typename T, bool QUANT>
 static int fwd_typed(const NormArgs& a, bool vec, cudaStream_t stream) {
     if (vec) {
-        if (a.dim <= 1024 * 8) return launch_fwd<T, 8, 1, QUANT>(a, threads_per_row(a.dim, 8, 1), stream);
-        return launch_fwd<T, 8, 2, QUANT>(a, threads_per_row(a.dim, 8, 2), stream);
+        // Few rows: as many threads as there are vectors (64 x 4096: 2.4 us with one vector per thread, 2.8 with two, 4.1 with four).  Many rows:
+        // blocks of about 300 threads, several per SM, so that some load while others reduce (4099 x 5120: 32.6 us against 38.2 with one
+        // vector per thread; 2000 x 8192: 28.8 with four against 33.0).
+        int nv = 1;
+        while (threads_per_row(a.dim, 8, nv) > (a.rows <= sm_count() ? 1024 : 320) && nv < 4) nv *= 2;
+        if (nv == 1) return launch_fwd<T, 8, 1, QUANT>(a, threads_per_row(a.dim, 8, 1), stream);
+        if (nv == 2) return launch_fwd<T, 8, 2, QUANT>(a, threads_per_row(a.dim, 8, 2), stream);
+        return launch_fwd<T, 8, 4, QUANT>(a, threads_per_row(a.dim, 8, 4), stream);
     }
     if (a.dim <= 1024 * 4) return launch_fwd<T, 1, 4, QUANT>(a, threads_per_row(a.dim, 1, 4), stream);
     return launch_fwd<T, 1, 16, QUANT>(a, threads_per_row(a.dim, 1, 16), stream);
@@ -286,24 +322,24 @@ static int fwd_typed(const NormArgs& a, bool vec, cudaStream_t stream) {
 // threads of a row and vectors a thread holds in the backward pass (dim <= NORM_MAX_DIM: at most 512 threads of 4 vectors)
 struct BwdShape { int nv, tpr; };
 static BwdShape norm_bwd_shape(int dim, bool vec) {
-    const int nv = vec ? (dim <= 512 * 16 ? 2 : 4) : (dim <= 1024 * 4 ? 4 : 16);
+    int nv = vec ? 1 : (dim <= 1024 * 4 ? 4 : 16);
+    while (vec && threads_per_row(dim, 8, nv) > 512) nv *= 2;
     return {nv, threads_per_row(dim, vec ? 8 : 1, nv)};
 }
 
 template <typename T>
 static int bwd_typed(const NormArgs& a, bool vec, int grid, cudaStream_t stream) {
     const BwdShape b = norm_bwd_shape(a.dim, vec);
-    void (*k)(const NormArgs, int) = vec ? (b.nv == 2 ? add_rms_norm_bwd_kernel<T, 8, 2> : add_rms_norm_bwd_kernel<T, 8, 4>)
+    void (*k)(const NormArgs, int) = vec ? (b.nv == 1 ? add_rms_norm_bwd_kernel<T, 8, 1> : b.nv == 2 ? add_rms_norm_bwd_kernel<T, 8, 2> : add_rms_norm_bwd_kernel<T, 8, 4>)
                                          : (b.nv == 4 ? add_rms_norm_bwd_kernel<T, 1, 4> : add_rms_norm_bwd_kernel<T, 1, 16>);
     return (int)launch_pdl(k, dim3(grid), dim3(b.tpr), 0, stream, a, b.tpr);
 }
 
-// about 1024 threads per SM walk the rows (the part of dw that each block leaves is dim floats); the same for both vector widths, so that
-// the workspace does not depend on the addresses
+// about 512 threads per SM walk the rows (8191 x 4096: 82.5 us with one block of 512 per SM, 87.8 with four; 4096 x 1024: 15.6 with four of 128);
+// the same for both vector widths, so that the workspace does not depend on the addresses
 static int norm_bwd_grid(long long rows, int dim) {
-    int per_sm = 1024 / norm_bwd_shape(dim, true).tpr;
+    int per_sm = 512 / norm_bwd_shape(dim, true).tpr;
     if (per_sm > 16) per_sm = 16;
-    if (per_sm < 3) per_sm = 3;
     const long long cap = (long long)sm_count() * per_sm;
     return (int)(rows < cap ? rows : cap);
 }

@@ -14,30 +14,45 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
-_PAIR = (torch.bfloat16, torch.float16)
-
+_PAIR = {torch.bfloat16: 0, torch.float16: 1}
 
 # ------------------------------------------------------------------ marshalling
-# The small calls of a decode step are bound by the host: addresses go to ctypes as plain integers, the stream is read without building a
-# Stream object, and the device is switched only when it is not the current one (23 us -> 12 us for a one-row norm).
+# The small calls of a decode step are bound by the host, so nothing here builds objects that a call does not need: addresses go to ctypes as
+# plain integers, the stream is read without a Stream object, contiguous tensors without a view, and the device is switched only when it is not
+# the current one (one-row norm 20 -> 10 us, one-row projection 20 -> 9 us).
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_functions: dict = {}
 
 
-def _call(name: str, dev: torch.device, *args) -> None:
-    fn = getattr(L.lib(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(dev.index))
+def _call(name: str, index: int, *args) -> None:
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(L.lib(), name)
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev.index))
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         L.check(rc, name)
 
 
-def _size(name: str, dev: torch.device, *args) -> int:
+def _size(name: str, index: int, *args) -> int:
     """A *_workspace_bytes function, which sizes for the current device."""
-    with torch.cuda.device(dev):
+    with torch.cuda.device(index):
         return getattr(L.lib(), name)(*args)
+
+
+def _device(x, *others) -> int:
+    """Index of the device that all tensors are on."""
+    index = x.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        L.require_cuda(x, *others)  # says what is wrong
+    return index
 
 
 def _ptr(t) -> int | None:
@@ -59,24 +74,38 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _mat(t: torch.Tensor | None, cols: int):
+    """(tensor to keep alive, address, row stride) of [..., cols] read as rows."""
+    if t is None:
+        return None, None, 0
+    if not t.is_contiguous():
+        t = _rows(t)
+        return t, t.data_ptr(), _ld(t)
+    return t, t.data_ptr(), cols
+
+
 def _pitch(n: int) -> int:
     return (n + 7) // 8 * 8
 
 
-def _tma_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """Rows as the tensor-core kernels fetch them: 16-byte aligned base, stride a multiple of 8 elements; other rows are copied once."""
-    t = _rows(t)
-    r, d = t.shape
-    if t.data_ptr() % 16 == 0:
-        if r == 1:
-            return t, _pitch(d)
-        ld = t.stride(0)
-        if ld % 8 == 0:
-            return t, ld
-    ld = _pitch(d)
-    out = torch.empty(r, ld, device=t.device, dtype=t.dtype)
-    _call("b200_align_rows", t.device, t.data_ptr(), _ld(t), out.data_ptr(), ld, r, d)
-    return out[:, :d], ld
+def _tma_rows(*ts: torch.Tensor):
+    """For each of one or two [..., K]: (rows, row stride) as the tensor-core kernels fetch them, 16-byte aligned base and a stride that is a multiple of 8
+    elements; other rows are copied, both matrices in one launch."""
+    out, todo = [], []
+    for t in ts:
+        t = _rows(t)
+        r, d = t.shape
+        ld = t.stride(0) if r > 1 else _pitch(d)
+        if t.data_ptr() % 16 or ld % 8:
+            ld = _pitch(d)
+            todo.append((t, torch.empty(r, ld, device=t.device, dtype=t.dtype)))
+            t = todo[-1][1][:, :d]
+        out.append((t, ld))
+    if todo:
+        (s0, d0), (s1, d1) = todo[0], todo[1] if len(todo) > 1 else (None, None)
+        _call("b200_align_rows", s0.get_device(), s0.data_ptr(), _ld(s0), d0.data_ptr(), s0.shape[0], _ptr(s1), _ld(s1) if s1 is not None else 0, _ptr(d1),
+              s1.shape[0] if s1 is not None else 0, s0.shape[1], d0.shape[1])
+    return out
 
 
 def _wants_grad(*tensors) -> bool:
@@ -89,7 +118,7 @@ def _wants_grad(*tensors) -> bool:
 
 def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K) -> torch.Tensor:
     out = torch.empty(M, N, device=a.device, dtype=a.dtype)
-    _call("b200_dense_product", a.device, a.data_ptr(), a_ld, a_mn, b.data_ptr(), b_ld, b_mn, L.DTYPES[a.dtype], M, N, K, out.data_ptr(), N)
+    _call("b200_dense_product", a.get_device(), a.data_ptr(), a_ld, a_mn, b.data_ptr(), b_ld, b_mn, _PAIR[a.dtype], M, N, K, out.data_ptr(), N)
     return out
 
 
@@ -99,21 +128,23 @@ def _scratch(nbytes: int, device) -> torch.Tensor | None:
 
 # ------------------------------------------------------------------ residual addition + rms norm
 def _norm_args(x, residual, weight, eps):
-    dev = L.require_cuda(x, residual, weight)
-    D = x.shape[-1]
-    assert x.dtype in L.DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}"
+    index, dt, D = _device(x, residual, weight), x.dtype, x.shape[-1]
+    assert dt in L.DTYPES, f"x must be bfloat16, float16 or float32, got {dt}"
     assert 1 <= D <= 16384, f"width {D} is outside 1..16384"
-    assert residual is None or (residual.dtype == x.dtype and residual.shape == x.shape), "residual must have the type and shape of x"
-    assert weight is None or (weight.shape == (D,) and weight.dtype in (x.dtype, torch.float32)), "weight must be [D], in x's type or float32"
+    assert residual is None or (residual.dtype is dt and residual.shape == x.shape), "residual must have the type and shape of x"
+    assert weight is None or (weight.shape == (D,) and (weight.dtype is dt or weight.dtype is torch.float32)), "weight must be [D], in x's type or float32"
     assert eps >= 0.0, "eps must not be negative"
-    return dev, D
+    return index, D
 
 
-def _norm_forward(x, residual, weight, eps, y, s, q8, sf):
-    """x, residual: 2-D rows; weight contiguous."""
-    rows, D = x.shape
-    _call("b200_add_rms_norm", x.device, x.data_ptr(), _ld(x), _ptr(residual), 0 if residual is None else _ld(residual), _ptr(weight),
-          weight is not None and weight.dtype is torch.float32, L.DTYPES[x.dtype], rows, D, eps, _ptr(y), _ptr(s), _ptr(q8), _ptr(sf))
+def _norm_forward(index, D, x, residual, weight, eps, y, s, q8, sf):
+    x, xp, x_ld = _mat(x, D)
+    residual, rp, r_ld = _mat(residual, D)
+    w_f32 = 0
+    if weight is not None:
+        w_f32 = weight.dtype is torch.float32
+        weight = weight.contiguous()
+    _call("b200_add_rms_norm", index, xp, x_ld, rp, r_ld, _ptr(weight), w_f32, L.DTYPES[x.dtype], x.numel() // D, D, eps, _ptr(y), _ptr(s), _ptr(q8), _ptr(sf))
 
 
 class _AddRmsNorm(torch.autograd.Function):
@@ -123,7 +154,7 @@ class _AddRmsNorm(torch.autograd.Function):
         y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
         s = torch.empty_like(y) if residual is not None else None
         wc = weight.contiguous() if weight is not None else None
-        _norm_forward(x2, r2, wc, eps, y, s, None, None)
+        _norm_forward(x.get_device(), x.shape[-1], x2, r2, wc, eps, y, s, None, None)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x2, r2, wc)
         ctx.eps, ctx.shape = eps, x.shape
@@ -142,9 +173,9 @@ class _AddRmsNorm(torch.autograd.Function):
         rows, D = x.shape
         ds = torch.empty(ctx.shape, device=dev, dtype=x.dtype)
         dw = torch.empty_like(w) if need_w else None
-        nb = _size("b200_add_rms_norm_bwd_workspace_bytes", dev, rows, D) if need_w else 0
+        nb = _size("b200_add_rms_norm_bwd_workspace_bytes", dev.index, rows, D) if need_w else 0
         ws = _scratch(nb, dev)
-        _call("b200_add_rms_norm_bwd", dev, x.data_ptr(), _ld(x), _ptr(r), 0 if r is None else _ld(r), _ptr(w), w is not None and w.dtype is torch.float32, L.DTYPES[x.dtype],
+        _call("b200_add_rms_norm_bwd", dev.index, x.data_ptr(), _ld(x), _ptr(r), 0 if r is None else _ld(r), _ptr(w), w is not None and w.dtype is torch.float32, L.DTYPES[x.dtype],
               rows, D, ctx.eps, gy.data_ptr(), _ptr(gs), ds.data_ptr(), _ptr(dw), _ptr(ws), nb)
         return ds if need_x else None, ds if need_r else None, dw, None
 
@@ -152,55 +183,52 @@ class _AddRmsNorm(torch.autograd.Function):
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """x, residual [..., D] bf16 | fp16 | fp32 -> (y, s): s = x + residual (x itself without a residual), y = s / sqrt(mean(s^2) + eps) * weight.
     The norm is taken of the unrounded fp32 sum.  weight [D] in x's type or fp32, or None for ones.  Differentiable."""
-    _norm_args(x, residual, weight, eps)
+    index, D = _norm_args(x, residual, weight, eps)
     if _wants_grad(x, residual, weight):
         out = _AddRmsNorm.apply(x, residual, weight, float(eps))
         return out if residual is not None else (out, x)
-    x2, r2 = _rows(x), _rows(residual) if residual is not None else None
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     s = torch.empty_like(y) if residual is not None else None
-    _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, float(eps), y, s, None, None)
-    return y, (s if residual is not None else x)
+    _norm_forward(index, D, x, residual, weight, float(eps), y, s, None, None)
+    return y, (x if s is None else s)
 
 
 def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6, want_y: bool = False):
     """The same norm with y in 8 bits -> (q8, sf, s[, y]): q8 uint8 e4m3 codes [rows, D], sf uint8 E8M0 [rows, D/32], rows = all leading
     dimensions together (what `cukern.mx_grouped` and `linear_act_q8` take); q8 * 2^(sf - 127) is y quantised per 32 from its fp32 value.  want_y:
     y in x's type too.  D % 32 == 0.  No gradient."""
-    dev, D = _norm_args(x, residual, weight, eps)
+    index, D = _norm_args(x, residual, weight, eps)
     assert D % 32 == 0, f"width {D} is not a multiple of 32"
     assert not _wants_grad(x, residual, weight), "add_rms_norm_quant has no gradient: use add_rms_norm, or detach its inputs"
-    x2, r2 = _rows(x), _rows(residual) if residual is not None else None
-    rows = x2.shape[0]
+    dev, rows = x.device, x.numel() // D
     q8 = torch.empty(rows, D, device=dev, dtype=torch.uint8)
     sf = torch.empty(rows, D // 32, device=dev, dtype=torch.uint8)
     s = torch.empty(x.shape, device=dev, dtype=x.dtype) if residual is not None else None
     y = torch.empty(x.shape, device=dev, dtype=x.dtype) if want_y else None
-    _norm_forward(x2, r2, weight.contiguous() if weight is not None else None, float(eps), y, s, q8, sf)
-    s = s if residual is not None else x
+    _norm_forward(index, D, x, residual, weight, float(eps), y, s, q8, sf)
+    if s is None:
+        s = x
     return (q8, sf, s, y) if want_y else (q8, sf, s)
 
 
 # ------------------------------------------------------------------ projection with bias, activation, residual
 def _linear_forward(x, x_ld, w, w_ld, bias, act, residual, out, z, z_ld):
-    M, K = x.shape
-    N = w.shape[0]
-    _call("b200_linear_act", x.device, x.data_ptr(), x_ld, w.data_ptr(), w_ld, L.DTYPES[x.dtype], M, N, K, _ptr(bias), act, _ptr(residual),
-          0 if residual is None else _ld(residual), out.data_ptr(), N, _ptr(z), z_ld)
+    (M, K), N = x.shape, w.shape[0]
+    residual, rp, r_ld = _mat(residual, N)
+    if bias is not None:
+        bias = bias.contiguous()
+    _call("b200_linear_act", x.get_device(), x.data_ptr(), x_ld, w.data_ptr(), w_ld, _PAIR[x.dtype], M, N, K, _ptr(bias), act, rp, r_ld, out.data_ptr(), N, _ptr(z), z_ld)
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, act, residual):
         N = w.shape[0]
-        x2, x_ld = _tma_rows(x)
-        w2, w_ld = _tma_rows(w)
-        r2 = _rows(residual) if residual is not None else None
-        b = bias.contiguous() if bias is not None else None
+        (x2, x_ld), (w2, w_ld) = _tma_rows(x, w)
         out = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
         z_ld = _pitch(N)
         z = torch.empty(x2.shape[0], z_ld, device=x.device, dtype=torch.float32) if act else None
-        _linear_forward(x2, x_ld, w2, w_ld, b, act, r2, out, z, z_ld)
+        _linear_forward(x2, x_ld, w2, w_ld, bias, act, residual, out, z, z_ld)
         ctx.save_for_backward(x2, w2, z)
         ctx.x_ld, ctx.w_ld, ctx.act, ctx.x_shape = x_ld, w_ld, act, x.shape
         return out
@@ -220,12 +248,12 @@ class _LinearAct(torch.autograd.Function):
             dz_ld = _pitch(N)
             dz = torch.empty(M, dz_ld, device=dev, dtype=x.dtype)
         if dz is not g2 or need_b:
-            nb = _size("b200_linear_act_bwd_workspace_bytes", dev, M, N) if need_b else 0
+            nb = _size("b200_linear_act_bwd_workspace_bytes", dev.index, M, N) if need_b else 0
             ws = _scratch(nb, dev)
-            _call("b200_linear_act_bwd", dev, g2.data_ptr(), _ld(g2), _ptr(z), _pitch(N), ctx.act, L.DTYPES[x.dtype], M, N, dz.data_ptr() if dz is not g2 else None, dz_ld,
+            _call("b200_linear_act_bwd", dev.index, g2.data_ptr(), _ld(g2), _ptr(z), _pitch(N), ctx.act, _PAIR[x.dtype], M, N, dz.data_ptr() if dz is not g2 else None, dz_ld,
                   _ptr(db), _ptr(ws), nb)
         if (need_x or need_w) and dz is g2:
-            dz, dz_ld = _tma_rows(g2)
+            ((dz, dz_ld),) = _tma_rows(g2)
         if need_x:
             dx = _product(dz, dz_ld, 0, w, ctx.w_ld, 1, M, K, N).view(ctx.x_shape)
         if need_w:
@@ -234,8 +262,9 @@ class _LinearAct(torch.autograd.Function):
 
 
 def _act_code(act) -> int:
-    assert act in L.ACTIVATIONS, f"act must be one of {sorted(a for a in L.ACTIVATIONS if a)} or None, got {act!r}"
-    return L.ACTIVATIONS[act]
+    code = L.ACTIVATIONS.get(act)
+    assert code is not None, f"act must be one of {sorted(a for a in L.ACTIVATIONS if a)} or None, got {act!r}"
+    return code
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -243,19 +272,19 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     (z Phi(z)) or "gelu_tanh".  fp32 accumulation, one rounding at the end.  Any K, N and number of rows; rows of x or w that do not start on
     16 bytes (a K that is no multiple of 8, an odd slice) are copied first.  Differentiable in x, w, bias and residual; with an activation a call
     that needs a gradient also keeps the pre-activation (N fp32 values per row)."""
-    L.require_cuda(x, w, bias, residual)
-    code = _act_code(act)
-    assert x.dtype in _PAIR and w.dtype == x.dtype and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
-    N, K = w.shape
-    assert x.dim() >= 1 and x.shape[-1] == K and K >= 1 and N >= 1, f"x {tuple(x.shape)} does not fit w {tuple(w.shape)}"
-    assert bias is None or (bias.shape == (N,) and bias.dtype == x.dtype), "bias must be [N] in x's type"
-    assert residual is None or (residual.shape == (*x.shape[:-1], N) and residual.dtype == x.dtype), "residual must have the type and shape of the result"
+    _device(x, w, bias, residual)
+    code, dt = _act_code(act), x.dtype
+    assert dt in _PAIR and w.dtype is dt and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
+    (N, K), xs = w.shape, x.shape
+    assert len(xs) >= 1 and xs[-1] == K and K >= 1 and N >= 1, f"x {tuple(xs)} does not fit w {tuple(w.shape)}"
+    shape = (*xs[:-1], N)
+    assert bias is None or (bias.dtype is dt and bias.shape == (N,)), "bias must be [N] in x's type"
+    assert residual is None or (residual.dtype is dt and residual.shape == shape), "residual must have the type and shape of the result"
     if _wants_grad(x, w, bias, residual):
         return _LinearAct.apply(x, w, bias, code, residual)
-    out = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
-    x2, x_ld = _tma_rows(x)
-    w2, w_ld = _tma_rows(w)
-    _linear_forward(x2, x_ld, w2, w_ld, bias.contiguous() if bias is not None else None, code, _rows(residual) if residual is not None else None, out, None, 0)
+    out = torch.empty(shape, device=x.device, dtype=dt)
+    (x2, x_ld), (w2, w_ld) = _tma_rows(x, w)
+    _linear_forward(x2, x_ld, w2, w_ld, bias, code, residual, out, None, 0)
     return out
 
 
@@ -264,23 +293,25 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
     """The projection on FP8 operands: x8 uint8 e4m3 [rows, K] + xsf uint8 E8M0 [rows, K/32] (`add_rms_norm_quant`, `cukern.mx_quantize_rows`), w8
     uint8 e4m3 [N, K] in natural k order (`w8.unpermute_k` of a W8's bytes) + s8 uint8 E8M0 [ceil(N/32), K/32].  bias [N], residual [rows, N] and
     the result bf16; products and sums in fp32.  K % 128 == 0.  No gradient."""
-    dev = L.require_cuda(x8, xsf, w8, s8, bias, residual)
-    code = _act_code(act)
-    assert all(t.dtype == torch.uint8 and t.dim() == 2 for t in (x8, xsf, w8, s8)), "x8, xsf, w8 and s8 are uint8 matrices"
+    index, code, u8 = _device(x8, xsf, w8, s8, bias, residual), _act_code(act), torch.uint8
+    assert x8.dtype is u8 and xsf.dtype is u8 and w8.dtype is u8 and s8.dtype is u8, "x8, xsf, w8 and s8 are uint8"
+    assert x8.dim() == 2 and w8.dim() == 2 and xsf.dim() == 2 and s8.dim() == 2, "x8, xsf, w8 and s8 are matrices"
     (M, K), N = x8.shape, w8.shape[0]
     assert K % 128 == 0 and K > 0 and w8.shape[1] == K and N >= 1, f"x8 {tuple(x8.shape)} / w8 {tuple(w8.shape)}: the widths must be equal and a multiple of 128"
-    assert xsf.shape == (M, K // 32) and s8.shape[0] == (N + 31) // 32 and s8.shape[1] >= K // 32, "one scale per 32 k: xsf [rows, K/32], s8 [ceil(N/32), K/32]"
-    assert bias is None or (bias.shape == (N,) and bias.dtype == torch.bfloat16), "bias must be bfloat16 [N]"
-    assert residual is None or (residual.shape == (M, N) and residual.dtype == torch.bfloat16), "residual must be bfloat16 [rows, N]"
+    s_rows, s_cols = s8.shape
+    assert xsf.shape == (M, K // 32) and s_rows == (N + 31) // 32 and s_cols >= K // 32, "one scale per 32 k: xsf [rows, K/32], s8 [ceil(N/32), K/32]"
+    assert bias is None or (bias.dtype is torch.bfloat16 and bias.shape == (N,)), "bias must be bfloat16 [N]"
+    assert residual is None or (residual.dtype is torch.bfloat16 and residual.shape == (M, N)), "residual must be bfloat16 [rows, N]"
     assert not _wants_grad(bias, residual), "linear_act_q8 has no gradient"
-    x8, xsf, w8, s8 = (t.contiguous() for t in (x8, xsf, w8, s8))
-    r2 = _rows(residual) if residual is not None else None
-    out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
-    b = bias.contiguous() if bias is not None else None
-    nb = _size("b200_linear_act_q8_workspace_bytes", dev, M, N, K)
-    ws = _scratch(nb, dev)
-    _call("b200_linear_act_q8", dev, x8.data_ptr(), xsf.data_ptr(), w8.data_ptr(), s8.data_ptr(), s8.shape[1], M, N, K, _ptr(b), code, _ptr(r2), 0 if r2 is None else _ld(r2),
-          out.data_ptr(), N, _ptr(ws), nb)
+    x8, xsf, w8, s8 = x8.contiguous(), xsf.contiguous(), w8.contiguous(), s8.contiguous()
+    residual, rp, r_ld = _mat(residual, N)
+    if bias is not None:
+        bias = bias.contiguous()
+    out = torch.empty(M, N, device=x8.device, dtype=torch.bfloat16)
+    nb = L.lib().b200_linear_act_q8_workspace_bytes(M, N, K)
+    ws = _scratch(nb, x8.device)
+    _call("b200_linear_act_q8", index, x8.data_ptr(), xsf.data_ptr(), w8.data_ptr(), s8.data_ptr(), s_cols, M, N, K, _ptr(bias), code, rp, r_ld, out.data_ptr(), N, _ptr(ws),
+          nb)
     return out
 
 
@@ -288,15 +319,14 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
 def _gated_forward(x, x_ld, w, w_ld, act, limit, out, gu, gu_ld):
     M, K = x.shape
     inter = w.shape[0] // 2
-    _call("b200_gated_linear", x.device, x.data_ptr(), x_ld, w.data_ptr(), w_ld, L.DTYPES[x.dtype], M, inter, K, act, limit, out.data_ptr(), inter, _ptr(gu), gu_ld)
+    _call("b200_gated_linear", x.get_device(), x.data_ptr(), x_ld, w.data_ptr(), w_ld, _PAIR[x.dtype], M, inter, K, act, limit, out.data_ptr(), inter, _ptr(gu), gu_ld)
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, act, limit):
         inter = w13.shape[0] // 2
-        x2, x_ld = _tma_rows(x)
-        w2, w_ld = _tma_rows(w13)
+        (x2, x_ld), (w2, w_ld) = _tma_rows(x, w13)
         out = torch.empty(*x.shape[:-1], inter, device=x.device, dtype=x.dtype)
         gu_ld = _pitch(2 * inter)
         gu = torch.empty(x2.shape[0], gu_ld, device=x.device, dtype=torch.float32)
@@ -315,7 +345,7 @@ class _GatedLinear(torch.autograd.Function):
         gu_ld = _pitch(n2)
         dx = dw = None
         dgu = torch.empty(M, gu_ld, device=dev, dtype=x.dtype)
-        _call("b200_gated_linear_bwd", dev, g2.data_ptr(), _ld(g2), gu.data_ptr(), gu_ld, ctx.act, ctx.limit, L.DTYPES[x.dtype], M, n2 // 2, dgu.data_ptr(), gu_ld)
+        _call("b200_gated_linear_bwd", dev.index, g2.data_ptr(), _ld(g2), gu.data_ptr(), gu_ld, ctx.act, ctx.limit, _PAIR[x.dtype], M, n2 // 2, dgu.data_ptr(), gu_ld)
         if need_x:
             dx = _product(dgu, gu_ld, 0, w, ctx.w_ld, 1, M, K, n2).view(ctx.x_shape)
         if need_w:
@@ -327,17 +357,16 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", l
     """act(min(g, limit)) * min(max(u, -limit), limit) with [g | u] = x w13^T, both projections and the product in one kernel: x [..., K], w13
     [2 * inter, K] (gate rows, then up rows: the layout of the expert weights), both bf16 or both fp16 -> [..., inter].  limit 0: no clamps.
     Differentiable in x and w13; a call that needs a gradient also keeps g and u (2 * inter fp32 values per row)."""
-    L.require_cuda(x, w13)
-    code = _act_code(act)
-    assert x.dtype in _PAIR and w13.dtype == x.dtype and w13.dim() == 2, "x and w13 must be both bfloat16 or both float16, w13 [2 * inter, K]"
-    n2, K = w13.shape
-    assert n2 >= 2 and n2 % 2 == 0 and K >= 1 and x.dim() >= 1 and x.shape[-1] == K, f"x {tuple(x.shape)} does not fit w13 {tuple(w13.shape)}"
+    _device(x, w13)
+    code, dt = _act_code(act), x.dtype
+    assert dt in _PAIR and w13.dtype is dt and w13.dim() == 2, "x and w13 must be both bfloat16 or both float16, w13 [2 * inter, K]"
+    (n2, K), xs = w13.shape, x.shape
+    assert n2 >= 2 and n2 % 2 == 0 and K >= 1 and len(xs) >= 1 and xs[-1] == K, f"x {tuple(xs)} does not fit w13 {tuple(w13.shape)}"
     assert limit >= 0.0, "limit must not be negative"
     if _wants_grad(x, w13):
         return _GatedLinear.apply(x, w13, code, float(limit))
-    out = torch.empty(*x.shape[:-1], n2 // 2, device=x.device, dtype=x.dtype)
-    x2, x_ld = _tma_rows(x)
-    w2, w_ld = _tma_rows(w13)
+    out = torch.empty((*xs[:-1], n2 // 2), device=x.device, dtype=dt)
+    (x2, x_ld), (w2, w_ld) = _tma_rows(x, w13)
     _gated_forward(x2, x_ld, w2, w_ld, code, float(limit), out, None, 0)
     return out
 

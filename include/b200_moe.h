@@ -356,7 +356,7 @@ int b200_ep_close(void* ptr);
  *
  * b200_linear_act: out[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + residual[M, N]; bias, residual, z may be NULL; z fp32 [M, N] receives the
  *   pre-activation (what the backward pass needs).  x and w start on 16 bytes and their strides are multiples of 8 (b200_align_rows makes
- *   such a copy of other tensors); everything else has any address and stride.
+ *   such copies of one or two other matrices of `cols` 16-bit values per row; rows2 = 0: one); everything else has any address and stride.
  * b200_linear_act_bwd: dz = gy * act'(z) [M, N] (or NULL) and dbias [N] = its column sums (or NULL; needs the workspace).
  * b200_gated_linear: out[M, inter] = act(min(g, limit)) * min(max(u, -limit), limit), [g | u] = x[M, K] w13[2 inter, K]^T, limit 0: no clamps;
  *   gu fp32 [M, 2 inter] (or NULL): g and u, unclamped, for the backward pass.
@@ -389,7 +389,8 @@ int b200_gated_linear_bwd(const void* gy, long long gy_ld, const float* gu, long
                           long long dgu_ld, cudaStream_t stream);
 int b200_dense_product(const void* a, long long a_ld, int a_mn, const void* b, long long b_ld, int b_mn, int dtype, int M, int N, int K, void* out, long long out_ld,
                        cudaStream_t stream);
-int b200_align_rows(const void* src, long long src_ld, void* dst, long long dst_ld, long long rows, int cols, cudaStream_t stream);
+int b200_align_rows(const void* src, long long src_ld, void* dst, long long rows, const void* src2, long long src2_ld, void* dst2, long long rows2, int cols,
+                    long long dst_ld, cudaStream_t stream);
 size_t b200_linear_act_q8_workspace_bytes(int M, int N, int K);
 int b200_linear_act_q8(const void* x8, const void* xsf, const void* w8, const void* s8, int s_cols, int M, int N, int K, const void* bias, int act, const void* residual,
                        long long r_ld, void* out, long long out_ld, void* workspace, size_t workspace_bytes, cudaStream_t stream);

@@ -105,9 +105,11 @@ def test_c_boundary_refusals(mods):
     assert dp(p, 64, 1, p, 64, 0, 0, 64, 64, 8, p, 64, n) == UNSUPPORTED
     assert dp(p, 60, 0, p, 64, 1, 0, 8, 64, 60, p, 64, n) == BAD_ALIGN
     assert dp(p, 64, 0, p, 56, 1, 0, 8, 64, 64, p, 64, n) == BAD_SHAPE
-    assert lib.b200_align_rows(p, 9, odd, 16, 4, 9, n) == BAD_ALIGN
-    assert lib.b200_align_rows(p, 9, p, 12, 4, 9, n) == BAD_ALIGN
-    assert lib.b200_align_rows(p, 9, p, 8, 4, 9, n) == BAD_SHAPE
+    assert lib.b200_align_rows(p, 9, odd, 4, n, 0, n, 0, 9, 16, n) == BAD_ALIGN
+    assert lib.b200_align_rows(p, 9, p, 4, n, 0, n, 0, 9, 12, n) == BAD_ALIGN
+    assert lib.b200_align_rows(p, 9, p, 4, n, 0, n, 0, 9, 8, n) == BAD_SHAPE
+    assert lib.b200_align_rows(p, 9, p, 4, n, 9, n, 2, 9, 16, n) == BAD_ARG
+    assert lib.b200_align_rows(n, 9, n, 0, n, 0, n, 0, 9, 16, n) == 0
     q8 = lib.b200_linear_act_q8
     assert q8(p, p, p, p, 2, 2, 8, 64, n, 0, n, 0, p, 8, p, 1 << 30, n) == BAD_SHAPE
     assert q8(p, p, p, p, 3, 2, 8, 128, n, 0, n, 0, p, 8, p, 1 << 30, n) == BAD_SHAPE
