@@ -31,10 +31,11 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, 
             float g[VEC];
             load_vec<T, VEC>(gy + r * gy_ld + c, g);
             if (z) {
-                float v[VEC];
+                float v[VEC], y[VEC], d[VEC];
                 load_vec<float, VEC>(z + r * z_ld + c, v);
+                act_bwd_n(act, v, y, d);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) g[i] *= act_bwd(act, v[i]).y;
+                for (int i = 0; i < VEC; ++i) g[i] *= d[i];
             }
             if (dz) store_vec<T, VEC>(dz + r * dz_ld + c, g);
 #pragma unroll
@@ -70,18 +71,20 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy
     load_vec<T, VEC>(gy + r * gy_ld + c, d);
     load_vec<float, VEC>(gu + r * gu_ld + c, g);
     load_vec<float, VEC>(gu + r * gu_ld + inter + c, u);
+    float pass_g[VEC], pass_u[VEC], a[VEC], da[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-        bool pass_g = true, pass_u = true;
+        pass_g[k] = pass_u[k] = d[k];
         if (limit > 0.f) {
-            pass_g = !(g[k] > limit);
-            pass_u = !(fabsf(u[k]) > limit);
-            if (!pass_g) g[k] = limit;
-            if (!pass_u) u[k] = copysignf(limit, u[k]);
+            if (g[k] > limit) { g[k] = limit; pass_g[k] = 0.f; }
+            if (fabsf(u[k]) > limit) { u[k] = copysignf(limit, u[k]); pass_u[k] = 0.f; }
         }
-        const float2 a = act_bwd(act, g[k]);
-        g[k] = pass_g ? d[k] * u[k] * a.y : 0.f;
-        u[k] = pass_u ? d[k] * a.x : 0.f;
+    }
+    act_bwd_n(act, g, a, da);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        g[k] = pass_g[k] * u[k] * da[k];
+        u[k] = pass_u[k] * a[k];
     }
     store_vec<T, VEC>(dgu + r * dgu_ld + c, g);
     store_vec<T, VEC>(dgu + r * dgu_ld + inter + c, u);

@@ -195,10 +195,7 @@ __device__ __forceinline__ void epilogue16(const FgParams& P, long long row, int
         for (int i = 0; i < 16; ++i) z[i] = __uint_as_float(acc[i]);
     }
     if (g.z_out) store16<float>(g.z_out + row * g.z_ld + col, P.vec_z, n, z);
-    if (g.act != ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = act_fwd(g.act, z[i]);
-    }
+    act_fwd_n(g.act, z);
     if (g.res) {
         float r[16];
         load16<T>(reinterpret_cast<const T*>(g.res) + row * g.res_ld + col, P.vec_res, n, r);
@@ -228,8 +225,9 @@ __device__ __forceinline__ void epilogue16_dual(const FgParams& P, long long row
             b[i] = b[i] > g.limit ? g.limit : (b[i] < -g.limit ? -g.limit : b[i]);
         }
     }
+    act_fwd_n(g.act, a);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) a[i] = act_fwd(g.act, a[i]) * b[i];
+    for (int i = 0; i < 16; ++i) a[i] *= b[i];
     store16<T>(reinterpret_cast<T*>(g.out) + row * g.out_ld + col, P.vec_out, n, a);
 }
 
