@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy
     pdl_launch_dependents();
     const int per_row = (inter + VEC - 1) / VEC;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long r = i / per_row;
+    const long long r = i <= 0xFFFFFFFFll ? (uint32_t)i / (uint32_t)per_row : i / per_row;  // a 64-bit division is 5 times the instructions
     if (r >= M) return;
     const int c = (int)(i - r * per_row) * VEC;
     float d[VEC], g[VEC], u[VEC];
@@ -254,7 +254,7 @@ extern "C" int b200_align_rows(const void* src, long long src_ld, void* dst, lon
 }
 
 extern "C" size_t b200_linear_act_q8_workspace_bytes(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= FS_MAX_M || N <= 0 || K <= 0) return 0;
     return ((size_t)M + N) * (size_t)K * 2;
 }
 
@@ -266,7 +266,15 @@ extern "C" int b200_linear_act_q8(const void* x8, const void* xsf, const void* w
     if (M == 0) return 0;
     if (!x8 || !xsf || !w8 || !s8 || !out) return ERR_BAD_ARG;
     if (out_ld < N || (residual && r_ld < N)) return ERR_BAD_SHAPE;
-    if (((uintptr_t)x8 & 15) || ((uintptr_t)w8 & 15)) return ERR_BAD_ALIGN;
+    if (((uintptr_t)x8 & 15) || ((uintptr_t)w8 & 15) || ((uintptr_t)xsf & 3)) return ERR_BAD_ALIGN;
+    if (M <= FS_MAX_M) {
+        FgArgs a{};
+        a.a.base = x8;
+        a.b.base = w8;
+        a.M = M; a.N = N; a.K = K;
+        a.act = act; a.bias = bias; a.res = residual; a.res_ld = r_ld; a.out = out; a.out_ld = out_ld;
+        return fs_q8_launch(a, (const uint8_t*)xsf, (const uint8_t*)s8, s_cols, stream);
+    }
     if (!workspace || workspace_bytes < b200_linear_act_q8_workspace_bytes(M, N, K)) return ERR_WORKSPACE;
     if ((uintptr_t)workspace & 15) return ERR_BAD_ALIGN;
     __nv_bfloat16 *xb = (__nv_bfloat16*)workspace, *wb = xb + (size_t)M * K;

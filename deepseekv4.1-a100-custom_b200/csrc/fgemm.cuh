@@ -37,6 +37,8 @@ int fg_launch(const FgArgs& a, cudaStream_t stream);
 // fstream.cu: the same for M <= FS_MAX_M, K-major operands
 constexpr int FS_MAX_M = 16;
 int fs_launch(const FgArgs& a, cudaStream_t stream);
+// e4m3 operands [M][K], [N][K] (dense) with E8M0 scales xsf [M][K/32], s8 [ceil(N/32)][s_cols]; K % 128 == 0, xsf 4-byte aligned
+int fs_q8_launch(const FgArgs& a, const uint8_t* xsf, const uint8_t* s8, int s_cols, cudaStream_t stream);
 int fg_device_error(int* out);  // device error word (a wait that ran out of time), read and cleared
 
 }  // namespace b200

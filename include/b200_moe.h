@@ -364,7 +364,7 @@ int b200_ep_close(void* ptr);
  * b200_dense_product: out[M, N] = sum_k A(m, k) B(n, k), A(i, k) at base[i * ld + k], or base[k * ld + i] with *_mn != 0: the products of the
  *   backward passes (dx = dz w: b_mn; dw = dz^T x: a_mn and b_mn) without transposed copies.  a_mn needs b_mn.  Alignment as b200_linear_act.
  * b200_linear_act_q8: the projection with x as e4m3 [M, K] + E8M0 [M, K/32] and w as e4m3 [N, K] (natural k order) + E8M0 [ceil(N/32), s_cols];
- *   bias, residual and out bf16.  K % 128 == 0, x8 and w8 16-byte aligned. */
+ *   bias, residual and out bf16.  K % 128 == 0, x8 and w8 16-byte, xsf 4-byte aligned. */
 #define B200_BF16 0
 #define B200_FP16 1
 #define B200_FP32 2
