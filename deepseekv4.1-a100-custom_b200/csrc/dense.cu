@@ -1,7 +1,5 @@
 // C entry points of the dense feed-forward operators: out = act(x W^T + bias) + residual and the gated product
 // act(x Wg^T) * (x Wu^T), with the element-wise halves of their backward passes.  The products are fgemm.cu's.
-#include <cuda_fp8.h>
-
 #include "b200_moe.h"
 #include "common.cuh"
 #include "dense.cuh"
@@ -107,25 +105,6 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const AlignRows m0, con
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? s[k] : 0;  // the rest of the last 16 bytes: zeros
     *reinterpret_cast<uint4*>((second ? m1.dst : m0.dst) + r * dst_ld + c) = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-}
-
-// e4m3 codes with one E8M0 scale per 32 k (row r's scales in row r >> row_shift of sf) -> bf16, exactly: 4 significant bits times a power of two
-__global__ void __launch_bounds__(256) dequant_rows_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int sf_ld, int row_shift, long long rows, int K,
-                                                           __nv_bfloat16* __restrict__ out) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int per_row = K / 16;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
-    if (r >= rows) return;
-    const int c = (int)(i - r * per_row) * 16;
-    const uint4 raw = *reinterpret_cast<const uint4*>(q + r * K + c);
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w}, e = sf[(r >> row_shift) * sf_ld + (c >> 5)];
-    const float s = e ? u32_as_f32(e << 23) : 5.877471754111438e-39f;  // 2^(e - 127)
-    float v[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(u[k >> 2] >> (8 * (k & 3))), __NV_E4M3))) * s;
-    store8<__nv_bfloat16>(out + r * K + c, *reinterpret_cast<const float(*)[8]>(&v[0]));
-    store8<__nv_bfloat16>(out + r * K + c + 8, *reinterpret_cast<const float(*)[8]>(&v[8]));
 }
 
 static bool ok16(const void* p, long long ld) { return !((uintptr_t)p & 15) && ld % 8 == 0; }  // rows start on 16 bytes (fp32: on 32)
@@ -254,8 +233,7 @@ extern "C" int b200_align_rows(const void* src, long long src_ld, void* dst, lon
 }
 
 extern "C" size_t b200_linear_act_q8_workspace_bytes(int M, int N, int K) {
-    if (M <= FS_MAX_M || N <= 0 || K <= 0) return 0;
-    return ((size_t)M + N) * (size_t)K * 2;
+    return M <= FS_MAX_M || N <= 0 || K <= 0 ? 0 : fg_sf_workspace_bytes(M, N, K / 2);
 }
 
 extern "C" int b200_linear_act_q8(const void* x8, const void* xsf, const void* w8, const void* s8, int s_cols, int M, int N, int K, const void* bias, int act,
@@ -267,21 +245,18 @@ extern "C" int b200_linear_act_q8(const void* x8, const void* xsf, const void* w
     if (!x8 || !xsf || !w8 || !s8 || !out) return ERR_BAD_ARG;
     if (out_ld < N || (residual && r_ld < N)) return ERR_BAD_SHAPE;
     if (((uintptr_t)x8 & 15) || ((uintptr_t)w8 & 15) || ((uintptr_t)xsf & 3)) return ERR_BAD_ALIGN;
-    if (M <= FS_MAX_M) {
-        FgArgs a{};
-        a.a.base = x8;
-        a.b.base = w8;
-        a.M = M; a.N = N; a.K = K;
-        a.act = act; a.bias = bias; a.res = residual; a.res_ld = r_ld; a.out = out; a.out_ld = out_ld;
-        return fs_q8_launch(a, (const uint8_t*)xsf, (const uint8_t*)s8, s_cols, stream);
-    }
+    FgArgs a{};
+    a.a.base = x8;
+    a.b.base = w8;
+    a.M = M; a.N = N; a.K = K;
+    a.act = act; a.bias = bias; a.res = residual; a.res_ld = r_ld; a.out = out; a.out_ld = out_ld;
+    if (M <= FS_MAX_M) return fs_q8_launch(a, (const uint8_t*)xsf, (const uint8_t*)s8, s_cols, stream);
     if (!workspace || workspace_bytes < b200_linear_act_q8_workspace_bytes(M, N, K)) return ERR_WORKSPACE;
     if ((uintptr_t)workspace & 15) return ERR_BAD_ALIGN;
-    __nv_bfloat16 *xb = (__nv_bfloat16*)workspace, *wb = xb + (size_t)M * K;
-    const long long bx = ((long long)M * (K / 16) + 255) / 256, bw = ((long long)N * (K / 16) + 255) / 256;
-    if (bx > 0x7FFFFFFFll || bw > 0x7FFFFFFFll) return ERR_TOO_LARGE;
-    cudaError_t e = launch_pdl(dequant_rows_kernel, dim3((unsigned)bx), dim3(256), 0, stream, (const uint8_t*)x8, (const uint8_t*)xsf, K / 32, 0, (long long)M, K, xb);
-    if (e == cudaSuccess) e = launch_pdl(dequant_rows_kernel, dim3((unsigned)bw), dim3(256), 0, stream, (const uint8_t*)w8, (const uint8_t*)s8, s_cols, 5, (long long)N, K, wb);
-    if (e != cudaSuccess) return (int)e;
-    return b200_linear_act(xb, K, wb, K, F_BF16, M, N, K, bias, act, residual, r_ld, out, out_ld, nullptr, 0, stream);
+    a.K = K / 2;
+    a.a.ld = a.b.ld = K / 2;
+    a.xsf = (const uint8_t*)xsf; a.s8 = (const uint8_t*)s8; a.s_cols = s_cols;
+    a.sf_workspace = workspace;
+    a.sf_workspace_bytes = workspace_bytes;
+    return fg_launch(a, stream);
 }

@@ -11,6 +11,8 @@
 // Every wait is bounded; one that runs out of time records a code in a device error word and the CTA runs to its end.
 #include "fgemm.cuh"
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "ftypes.cuh"
 #include "tc5.cuh"
@@ -26,10 +28,16 @@ constexpr int FG_SMEM = 224 * 1024;     // ring of stages
 
 // A stage holds two k blocks: a turn of the producer's loop costs it about 240 clocks plus 48 per copy whatever the copies' size (measured with
 // copies alone), a 256 x 256 pair tile is done with a k block in 512.
-template <int CG, int BN>
+// FP8 operands (MX): a k block is the same 128 bytes of a row, 128 values; a stage also holds the scale atoms of its two k blocks (tc5.cuh: 512 bytes for
+// 128 rows x 4 groups of 32 k): one of A and one per 128 rows of the whole B tile.
+template <int CG, int BN, bool MX>
 struct FgShape {
-    static constexpr uint32_t A_HALF = FG_BM * FG_BK * 2, B_ROWS = BN / CG, B_HALF = B_ROWS * FG_BK * 2, A_BYTES = 2 * A_HALF, B_BYTES = 2 * B_HALF, STAGE = A_BYTES + B_BYTES;
+    static constexpr uint32_t A_HALF = FG_BM * FG_BK * 2, B_ROWS = BN / CG, B_HALF = B_ROWS * FG_BK * 2, A_BYTES = 2 * A_HALF, B_BYTES = 2 * B_HALF;
+    static constexpr uint32_t SFB_ATOMS = (BN + 127) / 128, SFA_BYTES = MX ? 2 * 512 : 0, SFB_BYTES = MX ? 2 * SFB_ATOMS * 512 : 0;
+    static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
     static constexpr int NS = FG_SMEM / STAGE;
+    static constexpr uint32_t SF_COLS = 4 * (1 + SFB_ATOMS);  // TMEM columns of a k block's scales
+    static_assert(!MX || 2 * BN + NS * 2 * SF_COLS <= 512, "accumulators and scales must fit the tensor memory");
 };
 
 struct FgParams {
@@ -50,6 +58,24 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t adesc, uint64_t 
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(adesc), "l"(bdesc),
                      "r"(idesc), "r"(accumulate)
                      : "memory");
+}
+// block-scaled FP8: scales of A and B in TMEM, byte j of their columns chosen by the instruction descriptor
+template <int CG>
+__device__ __forceinline__ void tc_mma_mx8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa),
+            "r"(sfb)
+            : "memory");
+    else
+        tc_mma_mx(d, adesc, bdesc, idesc, sfa, sfb, accumulate);
+}
+// a scale atom of shared memory into 4 TMEM columns (CG = 2: in both CTAs, each from its own shared memory)
+template <int CG>
+__device__ __forceinline__ void tc_cp_atom(uint32_t taddr, uint64_t sdesc) {
+    if constexpr (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+    else tc_cp_sf(taddr, sdesc);
 }
 // the MMAs issued so far, when done, arrive on this barrier (CG = 2: on the barrier at the same place in both CTAs of the pair)
 template <int CG>
@@ -111,6 +137,11 @@ __device__ __forceinline__ uint32_t f16_idesc(int is_f16, int a_mn, int b_mn, in
 }
 
 struct FgPick { int cg, bn, split; };
+
+// instruction descriptor of kind::mxf8f6f4: both operands e4m3, K-major, E8M0 scales, byte j of the scale columns of both
+__device__ __forceinline__ uint32_t mx8_idesc(int m, int n, int j) {
+    return ((uint32_t)j << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) | ((uint32_t)j << 29);
+}
 
 // a wait whose phase is usually complete already: no look at the abort flag on that path
 __device__ __forceinline__ bool fg_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
@@ -287,9 +318,10 @@ __device__ __forceinline__ void epilogue_turned(const FgParams& P, float* buf, i
     }
 }
 
-template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool SPLIT>
-__global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P, const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b) {
-    using S = FgShape<CG, BN>;
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool SPLIT, bool MX>
+__global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P, const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                                                                const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb) {
+    using S = FgShape<CG, BN, MX>;
     constexpr int NS = S::NS;
     extern __shared__ __align__(1024) uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long bars[2 * NS + 4];  // full[s], empty[s], acc_full[2], acc_empty[2]
@@ -344,7 +376,7 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
                     const int k0 = st * 2 * FG_BK;
                     const bool two = 2 * st + 1 < P.k_blocks;  // the last stage may hold one k block
                     if (rank == 0)
-                        mbar_expect_tx(full0 + 8 * s, CG * ((A_MN || two ? S::A_BYTES : S::A_HALF) + (B_MN || two ? S::B_BYTES : S::B_HALF)));
+                        mbar_expect_tx(full0 + 8 * s, CG * ((A_MN || two ? S::A_BYTES : S::A_HALF) + (B_MN || two ? S::B_BYTES : S::B_HALF) + S::SFA_BYTES + S::SFB_BYTES));
                     auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
                         if constexpr (CG == 2) tma_load_2d_pair(dst, tm, x, y, bar);
                         else tma_load_2d(dst, tm, x, y, bar);
@@ -366,6 +398,10 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
                             load(db + S::B_HALF, &tm_b, k0 + FG_BK, n0);
                             if constexpr (CG == 1) load(db + S::B_HALF + S::B_HALF / 2, &tm_b, k0 + FG_BK, h1);
                         }
+                    }
+                    if constexpr (MX) {  // atoms [128 rows][k block] and [tile][k block][SFB_ATOMS]; behind the last k block whatever follows, unused
+                        load(db + S::B_BYTES, &tm_sfa, 0, (t.m * CG + (int)rank) * P.k_blocks + 2 * st);
+                        load(db + S::B_BYTES + S::SFA_BYTES, &tm_sfb, 0, (t.n * P.k_blocks + 2 * st) * (int)S::SFB_ATOMS);
                     }
                     if (++s == NS) { s = 0; ph ^= 1; }
                 }
@@ -396,9 +432,21 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
 #pragma unroll
                     for (int j = 0; j < 2 * FG_BK / 16; ++j) {
                         if (j == FG_BK / 16 && 2 * st + 1 >= P.k_blocks) break;
+                        if constexpr (MX) {  // 32 k of 8 bits are the same 32 bytes as 16 k of 16 bits
+                            const uint32_t sf = tmem + 2 * BN + (s * 2 + (j >> 2)) * S::SF_COLS;
+                            if ((j & 3) == 0) {
+                                const uint32_t atoms = ring0 + s * S::STAGE + S::A_BYTES + S::B_BYTES + (j >> 2) * 512, atoms_b = ring0 + s * S::STAGE + S::A_BYTES + S::B_BYTES + S::SFA_BYTES + (j >> 2) * S::SFB_ATOMS * 512;
+                                tc_cp_atom<CG>(sf, desc_sf_atom(atoms));
+#pragma unroll
+                                for (uint32_t q = 0; q < S::SFB_ATOMS; ++q) tc_cp_atom<CG>(sf + 4 + 4 * q, desc_sf_atom(atoms_b + q * 512));
+                            }
+                            const uint32_t o = (j & 3) * 2;
+                            tc_mma_mx8<CG>(d, da + o + (j >> 2) * (S::A_HALF >> 4), db + o + (j >> 2) * (S::B_HALF >> 4), mx8_idesc(FG_BM * CG, BN, j & 3), sf, sf + 4, st != st_lo || j != 0);
+                            continue;
+                        }
                         // 16 k further: 32 bytes inside the swizzled row (then the second k block), or two groups of 8 k (2048 bytes)
                         const uint32_t oa = A_MN ? j * 128 : (j & 3) * 2 + (j >> 2) * (S::A_HALF >> 4), ob = B_MN ? j * 128 : (j & 3) * 2 + (j >> 2) * (S::B_HALF >> 4);
-                        tc_mma_f16<CG>(d, da + oa, db + ob, idesc, st != st_lo || j != 0);
+                        if constexpr (!MX) tc_mma_f16<CG>(d, da + oa, db + ob, idesc, st != st_lo || j != 0);
                     }
                     tc_commit_pair<CG>(empty0 + 8 * s, lead);
                     if (++s == NS) { s = 0; ph ^= 1; }
@@ -412,10 +460,10 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
         for (int i = first; i < tiles; i += step, ++it) {
             const Tile t = tile_at(i, P.m_tiles, P.n_tiles);
             const uint32_t buf = it & 1, aph = (it >> 1) & 1;
+            const long long row = (long long)(t.m * CG + (int)rank) * FG_BM + q * 32 + lane;
             if (!fg_wait(bar_acc_full(buf), aph, &abort_flag, 21)) break;
             tc_fence_after();
             if constexpr (SPLIT) break;  // the parts of the tile are added below
-            const long long row = (long long)(t.m * CG + (int)rank) * FG_BM + q * 32 + lane;
             const uint32_t t0 = tmem + ((uint32_t)(q * 32) << 16) + buf * BN;
             if (g.dual) {
                 for (int c = half * (BN / 4); c < (half + 1) * (BN / 4); c += 16) {
@@ -550,21 +598,64 @@ static int fg_tmap(CUtensorMap* tm, const FgOperand& o, int is_f16, long long ro
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool SPLIT>
+// scale atoms as rows of 128 words, read `atoms` rows at a time
+static int fg_sf_tmap(CUtensorMap* tm, const void* base, long long rows, uint32_t atoms) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return (int)cudaErrorNotSupported;
+    cuuint64_t dims[2] = {128, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {512};
+    cuuint32_t box[2] = {128, atoms}, estr[2] = {1, 1};
+    CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+// E8M0 scales into atom order, one block of 128 threads per atom: byte (r % 32) * 16 + (r / 32) * 4 + g of an atom = scale of row r, group g of the
+// k block.  Atoms of x: [128 rows][k block], one row of scales per row; atoms of w: [tile of bn rows][k block][ceil(bn / 128)], one row of scales per
+// 32 rows.  Rows behind the last one borrow its scales (their products are not stored).
+__global__ void __launch_bounds__(128) fg_scale_atoms_kernel(const uint8_t* __restrict__ xsf, int M, const uint8_t* __restrict__ s8, int s_cols, int N, int k_blocks, int bn,
+                                                             int x_atoms, uint32_t* __restrict__ out) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int atom = blockIdx.x, r = threadIdx.x;
+    const uint8_t* src;
+    if (atom < x_atoms) {
+        const int mt = atom / k_blocks, kb = atom - mt * k_blocks;
+        src = xsf + (long long)min(mt * 128 + r, M - 1) * (k_blocks * 4) + kb * 4;
+    } else {
+        const int per = (bn + 127) / 128, i = atom - x_atoms, tk = i / per, nt = tk / k_blocks, kb = tk - nt * k_blocks;
+        src = s8 + (long long)(min(nt * bn + (i - tk * per) * 128 + r, N - 1) >> 5) * s_cols + kb * 4;
+    }
+    out[(long long)atom * 128 + (r & 31) * 4 + (r >> 5)] = src[0] | src[1] << 8 | src[2] << 16 | (uint32_t)src[3] << 24;
+}
+
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool SPLIT, bool MX>
 static int fg_run(FgParams& P, cudaStream_t stream) {
-    using S = FgShape<CG, BN>;
+    using S = FgShape<CG, BN, MX>;
     const FgArgs& g = P.g;
     P.m_tiles = (g.M + CG * FG_BM - 1) / (CG * FG_BM);
     P.n_tiles = g.dual ? (g.inter + BN / 2 - 1) / (BN / 2) : (g.N + BN - 1) / BN;
     P.k_blocks = (g.K + FG_BK - 1) / FG_BK;
     if ((long long)P.m_tiles * P.n_tiles > 0x0FFFFFFFll) return ERR_TOO_LARGE;
-    alignas(64) CUtensorMap ta, tb;
+    alignas(64) CUtensorMap ta, tb, tsa, tsb;
     int rc = fg_tmap(&ta, g.a, g.is_f16, g.M, g.K, FG_BM);
     if (!rc) rc = fg_tmap(&tb, g.b, g.is_f16, g.N, g.K, BN / 2);
+    tsa = tsb = ta;
+    if constexpr (MX) {
+        const long long xa = (long long)((g.M + 127) / 128) * P.k_blocks, wa = (long long)P.n_tiles * P.k_blocks * S::SFB_ATOMS;
+        if (xa + wa > 0x7FFFFFFFll) return ERR_TOO_LARGE;
+        if ((size_t)(xa + wa) * 512 > g.sf_workspace_bytes) return ERR_WORKSPACE;
+        if (!rc) rc = fg_sf_tmap(&tsa, g.sf_workspace, xa, 2);
+        if (!rc) rc = fg_sf_tmap(&tsb, (const uint8_t*)g.sf_workspace + xa * 512, wa, 2 * S::SFB_ATOMS);
+        if (rc) return rc;
+        const cudaError_t e = launch_pdl(fg_scale_atoms_kernel, dim3((unsigned)(xa + wa)), dim3(128), 0, stream, g.xsf, g.M, g.s8, g.s_cols, g.N, P.k_blocks, BN, (int)xa,
+                                         (uint32_t*)g.sf_workspace);
+        if (e != cudaSuccess) return (int)e;
+    }
     if (rc) return rc;
     const size_t smem = (size_t)S::NS * S::STAGE + 1024 + (P.turned ? FG_TURN_BYTES : 0);
-    constexpr int smem_max = S::NS * S::STAGE + 1024 + (BN == 192 ? 0 : FG_TURN_BYTES);
-    auto kernel = fg_gemm_kernel<T, CG, BN, A_MN, B_MN, SPLIT>;
+    constexpr int smem_max = S::NS * S::STAGE + 1024 + (BN == 192 || MX ? 0 : FG_TURN_BYTES);
+    auto kernel = fg_gemm_kernel<T, CG, BN, A_MN, B_MN, SPLIT, MX>;
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -587,40 +678,45 @@ static int fg_run(FgParams& P, cudaStream_t stream) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, P, ta, tb);
+    return (int)cudaLaunchKernelEx(&cfg, kernel, P, ta, tb, tsa, tsb);
 }
 
 template <typename T, int CG, int BN, bool SPLIT>
 static int fg_layouts(FgParams& P, cudaStream_t stream) {
+    if constexpr (BN != 256 && std::is_same<T, __nv_bfloat16>::value) {
+        if (P.g.xsf) return fg_run<T, CG, BN, false, false, SPLIT, true>(P, stream);
+    }
+    if (P.g.xsf) return ERR_UNSUPPORTED;
     if constexpr (BN == 192) {  // MN-major boxes are 64 rows wide: a pair's 96 rows of B are no multiple of that
-        return P.g.b.mn_major || P.g.a.mn_major ? ERR_UNSUPPORTED : fg_run<T, CG, BN, false, false, SPLIT>(P, stream);
+        return P.g.b.mn_major || P.g.a.mn_major ? ERR_UNSUPPORTED : fg_run<T, CG, BN, false, false, SPLIT, false>(P, stream);
     } else {
-        if (P.g.a.mn_major) return P.g.b.mn_major ? fg_run<T, CG, BN, true, true, SPLIT>(P, stream) : ERR_UNSUPPORTED;
-        return P.g.b.mn_major ? fg_run<T, CG, BN, false, true, SPLIT>(P, stream) : fg_run<T, CG, BN, false, false, SPLIT>(P, stream);
+        if (P.g.a.mn_major) return P.g.b.mn_major ? fg_run<T, CG, BN, true, true, SPLIT, false>(P, stream) : ERR_UNSUPPORTED;
+        return P.g.b.mn_major ? fg_run<T, CG, BN, false, true, SPLIT, false>(P, stream) : fg_run<T, CG, BN, false, false, SPLIT, false>(P, stream);
     }
 }
 
-// Which tile, and how many ways its k is split.  Each choice's time is estimated as (turns of the busiest CTA) x (stages of a tile) x (time of a
-// stage) + (start, end and last epilogue), the constants in us from measurements over 25 shapes between 64 x 4096 x 2048 and 8192 x 8192 x
-// 8192; e.g. measured 64 x 4096 x 4096: 1/128/4 13.9, 1/128/1 20.9, 2/256/1 25.7; 512 x 4096 x 4096: 2/256/2 21.3, 1/128/1 22.0, 1/128/4 47.5;
-// 1500 x 4096 x 4096: 2/192/1 41.9, 2/256/1 48.0, 1/128/1 55.9; 4096 x 12288 x 4096: 2/256/1 275, 2/192/1 290, 1/128/1 384.
+// Which tile, and how many ways its k is split.  Each choice's time is estimated as (turns of the busiest CTA) x (time of a tile: its stages' products, or
+// its epilogue where that is longer) + (start, end and last epilogue), the constants in us from measurements over 25 shapes between 64 x 4096 x 2048 and
+// 8192 x 8192 x 8192; e.g. measured 64 x 4096 x 4096: 1/128/4 13.9, 1/128/1 20.9, 2/256/1 25.7; 512 x 4096 x 4096: 2/256/2 21.3, 1/128/1 22.0,
+// 1/128/4 47.5; 1500 x 4096 x 4096: 2/192/1 41.9, 2/256/1 48.0, 1/128/1 55.9; 4096 x 12288 x 4096: 2/256/1 275, 2/192/1 290, 1/128/1 384.
+// FP8: 64 x 4096 x 4096: 1/128/4 14.4, 1/128/1 19.5, 2/192/1 24.1; 4096 x 12288 x 4096: 2/192/1 202, 1/128/1 249.
 static FgPick fg_pick(const FgParams& P) {
     const FgArgs& g = P.g;
-    static const struct { FgPick k; double stage, fixed; } choices[] = {
-        {{1, 128, 1}, .54, 4.0}, {{1, 128, 2}, .54, 7.5}, {{1, 128, 4}, .54, 8.5}, {{2, 128, 1}, .54, 4.5},  {{2, 128, 2}, .54, 8.0},
-        {{2, 192, 1}, .645, 5.5}, {{2, 256, 1}, .78, 6.5}, {{2, 256, 2}, .78, 10.0}};
+    static const struct { FgPick k; double stage, stage_mx, fixed, epi, epi_res; } choices[] = {
+        {{1, 128, 1}, .54, .76, 4.0, 2.5, 4.8}, {{1, 128, 2}, .54, .69, 7.5, 0, 0},      {{1, 128, 4}, .54, .69, 8.5, 0, 0},      {{2, 128, 1}, .54, .76, 4.5, 2.8, 5.0},
+        {{2, 128, 2}, .54, .70, 8.0, 0, 0},     {{2, 192, 1}, .645, .83, 5.5, 4.2, 7.5}, {{2, 256, 1}, .78, 0, 6.5, 5.0, 9.0}, {{2, 256, 2}, .78, 0, 10.0, 0, 0}};
     const int st = (g.K + 2 * FG_BK - 1) / (2 * FG_BK), sms = sm_count();
-    FgPick best{2, 256, 1};
+    FgPick best{1, 128, 1};
     double best_t = 1e30;
     for (const auto& c : choices) {
         const FgPick& k = c.k;
-        if (k.split > st || (k.bn == 192 && (g.a.mn_major || g.b.mn_major || P.turned))) continue;
+        if (k.split > st || (k.bn == 192 && (g.a.mn_major || g.b.mn_major || P.turned)) || (k.bn == 256 && g.xsf)) continue;
         const int cols = g.dual ? k.bn / 2 : k.bn, width = g.dual ? g.inter : g.N;
         const long long tiles = ((long long)g.M + k.cg * FG_BM - 1) / (k.cg * FG_BM) * ((width + cols - 1) / cols);
         const int groups = sms / (k.cg * k.split);
-        const double turns = (double)((tiles + groups - 1) / groups);
+        const double turns = (double)((tiles + groups - 1) / groups), stage = g.xsf ? c.stage_mx : c.stage, epi = g.res ? c.epi_res : c.epi;
         // persistent CTAs pay the fixed part once, clusters that split a tile once per turn
-        const double t = k.split > 1 ? turns * ((st + k.split - 1) / k.split * c.stage + c.fixed) : turns * st * c.stage + c.fixed;
+        const double t = k.split > 1 ? turns * ((st + k.split - 1) / k.split * stage + c.fixed) : turns * (st * stage > epi ? st * stage : epi) + c.fixed;
         if (t < best_t) { best_t = t; best = k; }
     }
     return best;
@@ -642,7 +738,7 @@ int fg_launch(const FgArgs& a, cudaStream_t stream) {
     if (a.dual && (a.N != 2 * a.inter || a.b.mn_major)) return ERR_BAD_SHAPE;
     if (((uintptr_t)a.a.base & 15) || ((uintptr_t)a.b.base & 15) || a.a.ld % 8 || a.b.ld % 8) return ERR_BAD_ALIGN;
     if (a.a.ld < (a.a.mn_major ? a.M : a.K) || a.b.ld < (a.b.mn_major ? a.N : a.K)) return ERR_BAD_SHAPE;
-    if (a.M <= FS_MAX_M && !a.a.mn_major && !a.b.mn_major) return fs_launch(a, stream);
+    if (a.M <= FS_MAX_M && !a.a.mn_major && !a.b.mn_major && !a.xsf) return fs_launch(a, stream);
     FgParams P{};
     P.g = a;
     auto vec = [](const void* p, long long ld_bytes) {
@@ -653,8 +749,13 @@ int fg_launch(const FgArgs& a, cudaStream_t stream) {
     P.vec_res = vec(a.res, a.res_ld * 2);
     P.vec_z = vec(a.z_out, a.dual ? a.z_ld * 4 | a.inter * 4 : a.z_ld * 4);
     P.vec_bias = vec(a.bias, 0);
-    P.turned = !P.vec_out || (a.res && !P.vec_res) || (a.z_out && !P.vec_z);
+    P.turned = !a.xsf && (!P.vec_out || (a.res && !P.vec_res) || (a.z_out && !P.vec_z));
     return a.is_f16 ? fg_dispatch<__half>(P, stream) : fg_dispatch<__nv_bfloat16>(P, stream);
+}
+
+size_t fg_sf_workspace_bytes(int M, int N, int K_pairs) {
+    const size_t kb = (K_pairs + FG_BK - 1) / FG_BK, x = ((size_t)M + 127) / 128, w128 = ((size_t)N + 127) / 128, w192 = ((size_t)N + 191) / 192 * 2;
+    return (x + (w128 > w192 ? w128 : w192)) * kb * 512;
 }
 
 int fg_device_error(int* out) {

@@ -1,6 +1,7 @@
 // Internal interface of the 16-bit tensor-core GEMM (fgemm.cu): bf16 x bf16 or fp16 x fp16 with fp32 accumulation.
 #pragma once
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 namespace b200 {
@@ -31,7 +32,14 @@ struct FgArgs {
     long long out_ld;
     float* z_out;
     long long z_ld;
+    // FP8 form (xsf given): A and B are e4m3 codes, their bases and K counted in pairs of codes (as the 16-bit values that TMA moves), with E8M0 scales
+    // xsf [M][K/16] and s8 [ceil(N/32)][s_cols]; K a multiple of 64 pairs; bias, residual and out bf16.  sf_workspace: fg_sf_workspace_bytes, 16-byte aligned
+    const uint8_t *xsf, *s8;
+    int s_cols;
+    void* sf_workspace;
+    size_t sf_workspace_bytes;
 };
+size_t fg_sf_workspace_bytes(int M, int N, int K_pairs);
 
 int fg_launch(const FgArgs& a, cudaStream_t stream);
 // fstream.cu: the same for M <= FS_MAX_M, K-major operands
