@@ -44,14 +44,12 @@ def _size(name: str, index: int, *args) -> int:
         return getattr(L.lib(), name)(*args)
 
 
-def _device(x, *others) -> int:
+def _device(a, b=None, c=None, d=None, e=None, f=None) -> int:
     """Index of the device that all tensors are on."""
-    index = x.get_device()
-    for t in others:
-        if t is not None and t.get_device() != index:
-            index = -1
-    if index < 0:
-        L.require_cuda(x, *others)  # says what is wrong
+    index = a.get_device()
+    if (index < 0 or b is not None and b.get_device() != index or c is not None and c.get_device() != index or d is not None and d.get_device() != index
+            or e is not None and e.get_device() != index or f is not None and f.get_device() != index):
+        L.require_cuda(a, b, c, d, e, f)  # says what is wrong
     return index
 
 
@@ -108,16 +106,25 @@ def _tma_rows(*ts: torch.Tensor):
     return out
 
 
-def _wants_grad(*tensors) -> bool:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
+def _operands(x: torch.Tensor, w: torch.Tensor, K: int):
+    """x [..., K] and w [N, K] as rows for the tensor-core kernels: (x, address, stride, w, address, stride); the tensors are kept for their memory."""
+    if not K & 7 and x.is_contiguous() and w.is_contiguous():
+        xp, wp = x.data_ptr(), w.data_ptr()
+        if not (xp | wp) & 15:
+            return x, xp, K, w, wp, K
+    (x, x_ld), (w, w_ld) = _tma_rows(x, w)
+    return x, x.data_ptr(), x_ld, w, w.data_ptr(), w_ld
 
 
-def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K) -> torch.Tensor:
-    out = torch.empty(M, N, device=a.device, dtype=a.dtype)
+_grad_enabled = torch.is_grad_enabled
+
+
+def _wants_grad(a, b=None, c=None, d=None) -> bool:
+    return _grad_enabled() and (a.requires_grad or b is not None and b.requires_grad or c is not None and c.requires_grad or d is not None and d.requires_grad)
+
+
+def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K, shape=None) -> torch.Tensor:
+    out = torch.empty(shape or (M, N), device=a.device, dtype=a.dtype)
     _call("b200_dense_product", a.get_device(), a.data_ptr(), a_ld, a_mn, b.data_ptr(), b_ld, b_mn, _PAIR[a.dtype], M, N, K, out.data_ptr(), N)
     return out
 
@@ -212,25 +219,29 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None = None, we
 
 
 # ------------------------------------------------------------------ projection with bias, activation, residual
-def _linear_forward(x, x_ld, w, w_ld, bias, act, residual, out, z, z_ld):
-    (M, K), N = x.shape, w.shape[0]
-    residual, rp, r_ld = _mat(residual, N)
+def _linear_forward(index, dt, ops, M, N, K, bias, act, residual, out, z, z_ld):
+    _, xp, x_ld, _, wp, w_ld = ops
+    bp, rp, r_ld = None, None, 0
     if bias is not None:
         bias = bias.contiguous()
-    _call("b200_linear_act", x.get_device(), x.data_ptr(), x_ld, w.data_ptr(), w_ld, _PAIR[x.dtype], M, N, K, _ptr(bias), act, rp, r_ld, out.data_ptr(), N, _ptr(z), z_ld)
+        bp = bias.data_ptr()
+    if residual is not None:
+        residual, rp, r_ld = _mat(residual, N)
+    _call("b200_linear_act", index, xp, x_ld, wp, w_ld, _PAIR[dt], M, N, K, bp, act, rp, r_ld, out.data_ptr(), N, _ptr(z), z_ld)
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, act, residual):
-        N = w.shape[0]
-        (x2, x_ld), (w2, w_ld) = _tma_rows(x, w)
-        out = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
+        N, K = w.shape
+        ops = _operands(x, w, K)
+        M = x.numel() // K
+        out = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
         z_ld = _pitch(N)
-        z = torch.empty(x2.shape[0], z_ld, device=x.device, dtype=torch.float32) if act else None
-        _linear_forward(x2, x_ld, w2, w_ld, bias, act, residual, out, z, z_ld)
-        ctx.save_for_backward(x2, w2, z)
-        ctx.x_ld, ctx.w_ld, ctx.act, ctx.x_shape = x_ld, w_ld, act, x.shape
+        z = torch.empty(M, z_ld, device=x.device, dtype=torch.float32) if act else None
+        _linear_forward(x.get_device(), x.dtype, ops, M, N, K, bias, act, residual, out, z, z_ld)
+        ctx.save_for_backward(ops[0], ops[3], z)
+        ctx.dims, ctx.lds, ctx.act, ctx.x_shape = (M, N, K), (ops[2], ops[5]), act, x.shape
         return out
 
     @staticmethod
@@ -238,26 +249,26 @@ class _LinearAct(torch.autograd.Function):
     def backward(ctx, gy):
         x, w, z = ctx.saved_tensors
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
-        (M, K), N, dev = x.shape, w.shape[0], x.device
+        (M, N, K), (x_ld, w_ld), dev, dt = ctx.dims, ctx.lds, x.device, x.dtype
         g2 = _rows(gy)
         dx = dw = db = None
         if need_b:
-            db = torch.empty(N, device=dev, dtype=x.dtype)
+            db = torch.empty(N, device=dev, dtype=dt)
         dz, dz_ld = g2, _ld(g2)
         if (need_x or need_w) and (ctx.act or N % 8):
             dz_ld = _pitch(N)
-            dz = torch.empty(M, dz_ld, device=dev, dtype=x.dtype)
+            dz = torch.empty(M, dz_ld, device=dev, dtype=dt)
         if dz is not g2 or need_b:
-            nb = _size("b200_linear_act_bwd_workspace_bytes", dev.index, M, N) if need_b else 0
+            nb = L.lib().b200_linear_act_bwd_workspace_bytes(M, N) if need_b else 0
             ws = _scratch(nb, dev)
-            _call("b200_linear_act_bwd", dev.index, g2.data_ptr(), _ld(g2), _ptr(z), _pitch(N), ctx.act, _PAIR[x.dtype], M, N, dz.data_ptr() if dz is not g2 else None, dz_ld,
+            _call("b200_linear_act_bwd", dev.index, g2.data_ptr(), _ld(g2), _ptr(z), _pitch(N), ctx.act, _PAIR[dt], M, N, dz.data_ptr() if dz is not g2 else None, dz_ld,
                   _ptr(db), _ptr(ws), nb)
         if (need_x or need_w) and dz is g2:
             ((dz, dz_ld),) = _tma_rows(g2)
         if need_x:
-            dx = _product(dz, dz_ld, 0, w, ctx.w_ld, 1, M, K, N).view(ctx.x_shape)
+            dx = _product(dz, dz_ld, 0, w, w_ld, 1, M, K, N, ctx.x_shape)
         if need_w:
-            dw = _product(dz, dz_ld, 1, x, ctx.x_ld, 1, N, K, M) if M else torch.zeros(N, K, device=dev, dtype=x.dtype)
+            dw = _product(dz, dz_ld, 1, x, x_ld, 1, N, K, M) if M else torch.zeros(N, K, device=dev, dtype=dt)
         return dx, dw, db, None, gy if need_r else None
 
 
@@ -272,19 +283,17 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     (z Phi(z)) or "gelu_tanh".  fp32 accumulation, one rounding at the end.  Any K, N and number of rows; rows of x or w that do not start on
     16 bytes (a K that is no multiple of 8, an odd slice) are copied first.  Differentiable in x, w, bias and residual; with an activation a call
     that needs a gradient also keeps the pre-activation (N fp32 values per row)."""
-    _device(x, w, bias, residual)
-    code, dt = _act_code(act), x.dtype
+    index, code, dt = _device(x, w, bias, residual), _act_code(act), x.dtype
     assert dt in _PAIR and w.dtype is dt and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
     (N, K), xs = w.shape, x.shape
-    assert len(xs) >= 1 and xs[-1] == K and K >= 1 and N >= 1, f"x {tuple(xs)} does not fit w {tuple(w.shape)}"
+    assert xs and xs[-1] == K and K >= 1 and N >= 1, f"x {tuple(xs)} does not fit w {tuple(w.shape)}"
     shape = (*xs[:-1], N)
     assert bias is None or (bias.dtype is dt and bias.shape == (N,)), "bias must be [N] in x's type"
     assert residual is None or (residual.dtype is dt and residual.shape == shape), "residual must have the type and shape of the result"
     if _wants_grad(x, w, bias, residual):
         return _LinearAct.apply(x, w, bias, code, residual)
     out = torch.empty(shape, device=x.device, dtype=dt)
-    (x2, x_ld), (w2, w_ld) = _tma_rows(x, w)
-    _linear_forward(x2, x_ld, w2, w_ld, bias, code, residual, out, None, 0)
+    _linear_forward(index, dt, _operands(x, w, K), x.numel() // K, N, K, bias, code, residual, out, None, 0)
     return out
 
 
@@ -302,13 +311,13 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
     assert xsf.shape == (M, K // 32) and s_rows == (N + 31) // 32 and s_cols >= K // 32, "one scale per 32 k: xsf [rows, K/32], s8 [ceil(N/32), K/32]"
     assert bias is None or (bias.dtype is torch.bfloat16 and bias.shape == (N,)), "bias must be bfloat16 [N]"
     assert residual is None or (residual.dtype is torch.bfloat16 and residual.shape == (M, N)), "residual must be bfloat16 [rows, N]"
-    assert not _wants_grad(bias, residual), "linear_act_q8 has no gradient"
+    assert not _wants_grad(x8, bias, residual), "linear_act_q8 has no gradient"
     x8, xsf, w8, s8 = x8.contiguous(), xsf.contiguous(), w8.contiguous(), s8.contiguous()
     residual, rp, r_ld = _mat(residual, N)
     if bias is not None:
         bias = bias.contiguous()
     out = torch.empty(M, N, device=x8.device, dtype=torch.bfloat16)
-    nb = L.lib().b200_linear_act_q8_workspace_bytes(M, N, K)
+    nb = L.lib().b200_linear_act_q8_workspace_bytes(M, N, K)  # none for decode-sized calls
     ws = _scratch(nb, x8.device)
     _call("b200_linear_act_q8", index, x8.data_ptr(), xsf.data_ptr(), w8.data_ptr(), s8.data_ptr(), s_cols, M, N, K, _ptr(bias), code, rp, r_ld, out.data_ptr(), N, _ptr(ws),
           nb)
@@ -316,23 +325,24 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
 
 
 # ------------------------------------------------------------------ gated projection
-def _gated_forward(x, x_ld, w, w_ld, act, limit, out, gu, gu_ld):
-    M, K = x.shape
-    inter = w.shape[0] // 2
-    _call("b200_gated_linear", x.get_device(), x.data_ptr(), x_ld, w.data_ptr(), w_ld, _PAIR[x.dtype], M, inter, K, act, limit, out.data_ptr(), inter, _ptr(gu), gu_ld)
+def _gated_forward(index, dt, ops, M, inter, K, act, limit, out, gu, gu_ld):
+    _, xp, x_ld, _, wp, w_ld = ops
+    _call("b200_gated_linear", index, xp, x_ld, wp, w_ld, _PAIR[dt], M, inter, K, act, limit, out.data_ptr(), inter, _ptr(gu), gu_ld)
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, act, limit):
-        inter = w13.shape[0] // 2
-        (x2, x_ld), (w2, w_ld) = _tma_rows(x, w13)
-        out = torch.empty(*x.shape[:-1], inter, device=x.device, dtype=x.dtype)
-        gu_ld = _pitch(2 * inter)
-        gu = torch.empty(x2.shape[0], gu_ld, device=x.device, dtype=torch.float32)
-        _gated_forward(x2, x_ld, w2, w_ld, act, limit, out, gu, gu_ld)
-        ctx.save_for_backward(x2, w2, gu)
-        ctx.x_ld, ctx.w_ld, ctx.act, ctx.limit, ctx.x_shape = x_ld, w_ld, act, limit, x.shape
+        n2, K = w13.shape
+        inter = n2 // 2
+        ops = _operands(x, w13, K)
+        M = x.numel() // K
+        out = torch.empty((*x.shape[:-1], inter), device=x.device, dtype=x.dtype)
+        gu_ld = _pitch(n2)
+        gu = torch.empty(M, gu_ld, device=x.device, dtype=torch.float32)
+        _gated_forward(x.get_device(), x.dtype, ops, M, inter, K, act, limit, out, gu, gu_ld)
+        ctx.save_for_backward(ops[0], ops[3], gu)
+        ctx.dims, ctx.lds, ctx.act, ctx.limit, ctx.x_shape = (M, n2, K), (ops[2], ops[5]), act, limit, x.shape
         return out
 
     @staticmethod
@@ -340,16 +350,16 @@ class _GatedLinear(torch.autograd.Function):
     def backward(ctx, gy):
         x, w, gu = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        (M, K), n2, dev = x.shape, w.shape[0], x.device
+        (M, n2, K), (x_ld, w_ld), dev, dt = ctx.dims, ctx.lds, x.device, x.dtype
         g2 = _rows(gy)
         gu_ld = _pitch(n2)
         dx = dw = None
-        dgu = torch.empty(M, gu_ld, device=dev, dtype=x.dtype)
-        _call("b200_gated_linear_bwd", dev.index, g2.data_ptr(), _ld(g2), gu.data_ptr(), gu_ld, ctx.act, ctx.limit, _PAIR[x.dtype], M, n2 // 2, dgu.data_ptr(), gu_ld)
+        dgu = torch.empty(M, gu_ld, device=dev, dtype=dt)
+        _call("b200_gated_linear_bwd", dev.index, g2.data_ptr(), _ld(g2), gu.data_ptr(), gu_ld, ctx.act, ctx.limit, _PAIR[dt], M, n2 // 2, dgu.data_ptr(), gu_ld)
         if need_x:
-            dx = _product(dgu, gu_ld, 0, w, ctx.w_ld, 1, M, K, n2).view(ctx.x_shape)
+            dx = _product(dgu, gu_ld, 0, w, w_ld, 1, M, K, n2, ctx.x_shape)
         if need_w:
-            dw = _product(dgu, gu_ld, 1, x, ctx.x_ld, 1, n2, K, M) if M else torch.zeros(n2, K, device=dev, dtype=x.dtype)
+            dw = _product(dgu, gu_ld, 1, x, x_ld, 1, n2, K, M) if M else torch.zeros(n2, K, device=dev, dtype=dt)
         return dx, dw, None, None
 
 
@@ -357,17 +367,15 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", l
     """act(min(g, limit)) * min(max(u, -limit), limit) with [g | u] = x w13^T, both projections and the product in one kernel: x [..., K], w13
     [2 * inter, K] (gate rows, then up rows: the layout of the expert weights), both bf16 or both fp16 -> [..., inter].  limit 0: no clamps.
     Differentiable in x and w13; a call that needs a gradient also keeps g and u (2 * inter fp32 values per row)."""
-    _device(x, w13)
-    code, dt = _act_code(act), x.dtype
+    index, code, dt = _device(x, w13), _act_code(act), x.dtype
     assert dt in _PAIR and w13.dtype is dt and w13.dim() == 2, "x and w13 must be both bfloat16 or both float16, w13 [2 * inter, K]"
     (n2, K), xs = w13.shape, x.shape
-    assert n2 >= 2 and n2 % 2 == 0 and K >= 1 and len(xs) >= 1 and xs[-1] == K, f"x {tuple(xs)} does not fit w13 {tuple(w13.shape)}"
+    assert n2 >= 2 and n2 % 2 == 0 and K >= 1 and xs and xs[-1] == K, f"x {tuple(xs)} does not fit w13 {tuple(w13.shape)}"
     assert limit >= 0.0, "limit must not be negative"
     if _wants_grad(x, w13):
         return _GatedLinear.apply(x, w13, code, float(limit))
     out = torch.empty((*xs[:-1], n2 // 2), device=x.device, dtype=dt)
-    (x2, x_ld), (w2, w_ld) = _tma_rows(x, w13)
-    _gated_forward(x2, x_ld, w2, w_ld, code, float(limit), out, None, 0)
+    _gated_forward(index, dt, _operands(x, w13, K), x.numel() // K, n2 // 2, K, code, float(limit), out, None, 0)
     return out
 
 
