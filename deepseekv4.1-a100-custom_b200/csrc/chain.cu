@@ -17,6 +17,7 @@ namespace b200 {
 
 int p2p_device_error(int* out);  // p2p.cu
 int fg_device_error(int* out);   // fgemm.cu
+int norm_device_error(int* out); // norm.cu
 
 constexpr int ROUTE_THREADS = 128;
 static_assert(ROUTE_THREADS == GATE_BLOCK_THREADS, "the block router is written for the routing kernels' block size");
@@ -1158,11 +1159,12 @@ extern "C" int b200_device_error(int* code, cudaStream_t stream) {
     int wm = 0, pp = 0;
     if ((rc = wm_device_error(&wm))) return rc;
     if ((rc = p2p_device_error(&pp))) return rc;
-    int fg = 0;
+    int fg = 0, nm = 0;
     if ((rc = fg_device_error(&fg))) return rc;
+    if ((rc = norm_device_error(&nm))) return rc;
     // prefill tensor-core kernel 11..41, streaming kernels 1001..1091, decode weight-stream kernel 2011..2042, messaging waits 3001..3004,
-    // 16-bit / FP8 GEMMs of the dense operators 4001..
-    *code = mx ? mx : (sk ? 1000 + sk : (wm ? 2000 + wm : (pp ? 3000 + pp : (fg ? 4000 + fg : 0))));
+    // 16-bit / FP8 GEMMs of the dense operators 4001..4021, norm backward 5001
+    *code = mx ? mx : (sk ? 1000 + sk : (wm ? 2000 + wm : (pp ? 3000 + pp : (fg ? 4000 + fg : (nm ? 5000 + nm : 0)))));
     return 0;
 }
 

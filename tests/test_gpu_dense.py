@@ -74,7 +74,7 @@ def norm64(x, r, w, eps):
     return s, n, n * (w.double() if w is not None else 1)
 
 
-NORM_SHAPES = [(1, 4096), (5, 1), (3, 7), (4, 32), (9, 250), (7, 512), (2, 1000), (3, 4097), (6, 5120), (2, 8192), (2, 8200), (3, 16384), (700, 64), (1500, 264)]
+NORM_SHAPES = [(1, 4096), (5, 1), (3, 7), (4, 32), (9, 250), (7, 512), (2, 1000), (3, 4097), (6, 5120), (2, 8192), (2, 8200), (3, 16384), (700, 64), (1500, 264), (400, 5120), (310, 8192)]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
@@ -150,7 +150,7 @@ def check_codes(q8, sf, y64, scale_rel):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("rows,dim", [(1, 4096), (3, 32), (70, 96), (5, 1024), (4099, 160), (2, 5120), (2, 16384)])
+@pytest.mark.parametrize("rows,dim", [(1, 4096), (3, 32), (70, 96), (5, 1024), (4099, 160), (2, 5120), (2, 16384), (400, 4128), (330, 8192)])
 def test_norm_quant(D, dev, dt, rows, dim):
     t = TYPES[dt]
     x, r = randn((rows, dim), 21, dev, t), randn((rows, dim), 22, dev, t)
