@@ -40,8 +40,11 @@ def _call(name: str, index: int, *args) -> None:
 
 def _size(name: str, index: int, *args) -> int:
     """A *_workspace_bytes function, which sizes for the current device."""
+    fn = getattr(L.lib(), name)
+    if index == _current_device():
+        return fn(*args)
     with torch.cuda.device(index):
-        return getattr(L.lib(), name)(*args)
+        return fn(*args)
 
 
 def _device(a, b=None, c=None, d=None, e=None, f=None) -> int:
@@ -86,24 +89,30 @@ def _pitch(n: int) -> int:
     return (n + 7) // 8 * 8
 
 
-def _tma_rows(*ts: torch.Tensor):
-    """For each of one or two [..., K]: (rows, row stride) as the tensor-core kernels fetch them, 16-byte aligned base and a stride that is a multiple of 8
-    elements; other rows are copied, both matrices in one launch."""
-    out, todo = [], []
-    for t in ts:
-        t = _rows(t)
-        r, d = t.shape
-        ld = t.stride(0) if r > 1 else _pitch(d)
-        if t.data_ptr() % 16 or ld % 8:
-            ld = _pitch(d)
-            todo.append((t, torch.empty(r, ld, device=t.device, dtype=t.dtype)))
-            t = todo[-1][1][:, :d]
-        out.append((t, ld))
-    if todo:
-        (s0, d0), (s1, d1) = todo[0], todo[1] if len(todo) > 1 else (None, None)
-        _call("b200_align_rows", s0.get_device(), s0.data_ptr(), _ld(s0), d0.data_ptr(), s0.shape[0], _ptr(s1), _ld(s1) if s1 is not None else 0, _ptr(d1),
-              s1.shape[0] if s1 is not None else 0, s0.shape[1], d0.shape[1])
-    return out
+def _fetchable(t: torch.Tensor, ld: int) -> bool:
+    """Rows as the tensor-core kernels fetch them: 16-byte aligned base, a stride that is a multiple of 8 elements."""
+    return not (t.data_ptr() & 15 or ld & 7)
+
+
+def _aligned(x: torch.Tensor, w: torch.Tensor | None, K: int):
+    """Copies of the rows x [R, K] and w [N, K] (w may be None) that the kernels can fetch, both in one launch: (scratch, rows of x, row stride)."""
+    ld = _pitch(K)
+    rx, rw = x.shape[0], 0 if w is None else w.shape[0]
+    buf = torch.empty(rx + rw, ld, device=x.device, dtype=x.dtype)
+    p = buf.data_ptr()
+    _call("b200_align_rows", x.get_device(), x.data_ptr(), _ld(x), p, rx, _ptr(w), 0 if w is None else _ld(w), p + 2 * rx * ld, rw, K, ld)
+    return buf, rx, ld
+
+
+def _tma_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """One matrix as fetchable rows: (rows, row stride)."""
+    t = _rows(t)
+    r, d = t.shape
+    ld = t.stride(0) if r > 1 else _pitch(d)
+    if _fetchable(t, ld):
+        return t, ld
+    buf, _, ld = _aligned(t, None, d)
+    return buf[:, :d], ld
 
 
 def _operands(x: torch.Tensor, w: torch.Tensor, K: int):
@@ -112,7 +121,19 @@ def _operands(x: torch.Tensor, w: torch.Tensor, K: int):
         xp, wp = x.data_ptr(), w.data_ptr()
         if not (xp | wp) & 15:
             return x, xp, K, w, wp, K
-    (x, x_ld), (w, w_ld) = _tma_rows(x, w)
+    x, w = _rows(x), _rows(w)
+    x_ld, w_ld = x.stride(0) if x.shape[0] > 1 else _pitch(K), w.stride(0) if w.shape[0] > 1 else _pitch(K)
+    okx, okw = _fetchable(x, x_ld), _fetchable(w, w_ld)
+    if okx and okw:
+        return x, x.data_ptr(), x_ld, w, w.data_ptr(), w_ld
+    if okx:
+        w, _, w_ld = _aligned(w, None, K)
+    elif okw:
+        x, _, x_ld = _aligned(x, None, K)
+    else:
+        buf, rx, x_ld = _aligned(x, w, K)
+        w_ld = x_ld
+        x, w = buf[:rx], buf[rx:]
     return x, x.data_ptr(), x_ld, w, w.data_ptr(), w_ld
 
 
@@ -127,6 +148,11 @@ def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K, shape=None) -> torch.Tensor:
     out = torch.empty(shape or (M, N), device=a.device, dtype=a.dtype)
     _call("b200_dense_product", a.get_device(), a.data_ptr(), a_ld, a_mn, b.data_ptr(), b_ld, b_mn, _PAIR[a.dtype], M, N, K, out.data_ptr(), N)
     return out
+
+
+def _once(cls, ctx, *gs):
+    """The gradients under torch's guard against a second differentiation (its wrapper costs more than the launches of a small step)."""
+    return once_differentiable(cls.gradients)(ctx, *gs)
 
 
 def _scratch(nbytes: int, device) -> torch.Tensor | None:
@@ -168,8 +194,13 @@ class _AddRmsNorm(torch.autograd.Function):
         return (y, s) if residual is not None else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gy, gs=None):
+        if _grad_enabled():  # create_graph: torch marks the gradients as not differentiable again
+            return _once(_AddRmsNorm, ctx, gy, gs)
+        return _AddRmsNorm.gradients(ctx, gy, gs)
+
+    @staticmethod
+    def gradients(ctx, gy, gs=None):
         x, r, w = ctx.saved_tensors
         need_x, need_r, need_w, _ = ctx.needs_input_grad
         if gy is None:  # the normed output was not used
@@ -245,8 +276,13 @@ class _LinearAct(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gy):
+        if _grad_enabled():
+            return _once(_LinearAct, ctx, gy)
+        return _LinearAct.gradients(ctx, gy)
+
+    @staticmethod
+    def gradients(ctx, gy):
         x, w, z = ctx.saved_tensors
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
         (M, N, K), (x_ld, w_ld), dev, dt = ctx.dims, ctx.lds, x.device, x.dtype
@@ -264,7 +300,7 @@ class _LinearAct(torch.autograd.Function):
             _call("b200_linear_act_bwd", dev.index, g2.data_ptr(), _ld(g2), _ptr(z), _pitch(N), ctx.act, _PAIR[dt], M, N, dz.data_ptr() if dz is not g2 else None, dz_ld,
                   _ptr(db), _ptr(ws), nb)
         if (need_x or need_w) and dz is g2:
-            ((dz, dz_ld),) = _tma_rows(g2)
+            dz, dz_ld = _tma_rows(g2)
         if need_x:
             dx = _product(dz, dz_ld, 0, w, w_ld, 1, M, K, N, ctx.x_shape)
         if need_w:
@@ -346,8 +382,13 @@ class _GatedLinear(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gy):
+        if _grad_enabled():
+            return _once(_GatedLinear, ctx, gy)
+        return _GatedLinear.gradients(ctx, gy)
+
+    @staticmethod
+    def gradients(ctx, gy):
         x, w, gu = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         (M, n2, K), (x_ld, w_ld), dev, dt = ctx.dims, ctx.lds, x.device, x.dtype

@@ -641,3 +641,16 @@ def test_two_captured_graphs(D, dev):
 
 def test_no_device_error_left(mods, dev):
     assert mods.cukern.device_error(dev) == 0
+
+
+def test_no_second_derivatives(D, dev):
+    """Gradients with create_graph are the same values and refuse to be differentiated again."""
+    x, w = randn((8, 64), 1, dev, torch.bfloat16).requires_grad_(True), randn((16, 64), 2, dev, torch.bfloat16).requires_grad_(True)
+    n, w13 = randn((64,), 3, dev, torch.bfloat16).requires_grad_(True), randn((32, 64), 4, dev, torch.bfloat16).requires_grad_(True)
+    for f, leaves in ((lambda: D.linear_act(x, w, None, "gelu"), (x, w)), (lambda: D.gated_linear(x, w13), (x, w13)), (lambda: D.add_rms_norm(x, None, n)[0], (x, n))):
+        y = f()
+        plain = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+        graph = torch.autograd.grad(y, leaves, torch.ones_like(y), create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+            torch.autograd.grad(graph[0].float().sum(), leaves[1])
