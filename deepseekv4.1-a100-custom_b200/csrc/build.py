@@ -1,8 +1,9 @@
-"""Compile the CUDA sources of this package for sm_100a into one shared library, in-tree.
+"""Compile the CUDA sources of this package for sm_100a into one shared library, in-tree, and the Python extension that shortens the way to
+the dense operators' forward calls.
 
     python deepseekv4.1-a100-custom_b200/csrc/build.py [--force] [--verbose]
 
-Produces csrc/libb200moe.so (git-ignored).  nvcc cross-compiles without a GPU.
+Produces csrc/libb200moe.so and csrc/_fastcall.so (git-ignored).  nvcc cross-compiles without a GPU.
 """
 from __future__ import annotations
 
@@ -16,6 +17,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 LIB = os.path.join(HERE, "libb200moe.so")
+FASTCALL = os.path.join(HERE, "_fastcall.so")
 NVCC = os.environ.get("B200MOE_NVCC", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -50,7 +52,33 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def build_fastcall(force: bool = False) -> str:
+    """fastcall.cpp against the installed torch (host code only)."""
+    src = os.path.join(HERE, "fastcall.cpp")
+    if not force and os.path.exists(FASTCALL) and all(os.path.getmtime(d) <= os.path.getmtime(FASTCALL) for d in (src, os.path.abspath(__file__))):
+        return FASTCALL
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+    inc = [*ext.include_paths(), sysconfig.get_paths()["include"], os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f for i in inc for f in ("-isystem", i)), src,
+           "-o", FASTCALL, *(f"-L{d}" for d in ext.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    return FASTCALL
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    with cf.ThreadPoolExecutor(max_workers=1) as side:  # beside nvcc
+        fast = side.submit(build_fastcall, force)
+        lib = build_library(force, verbose)
+        fast.result()
+    return lib
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB
     os.makedirs(os.path.join(HERE, "_obj"), exist_ok=True)

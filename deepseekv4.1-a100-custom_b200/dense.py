@@ -9,12 +9,17 @@ gradient.  A captured backward pass needs what torch asks of any: capture it on 
 same leaves first."""
 from __future__ import annotations
 
+import ctypes
+import importlib.util
+import os
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
 _PAIR = {torch.bfloat16: 0, torch.float16: 1}
+_ACT = L.ACTIVATIONS
 
 # ------------------------------------------------------------------ marshalling
 # The small calls of a decode step are bound by the host, so nothing here builds objects that a call does not need: addresses go to ctypes as
@@ -23,6 +28,25 @@ _PAIR = {torch.bfloat16: 0, torch.float16: 1}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _functions: dict = {}
+
+
+_fast = None  # csrc/fastcall.cpp, bound on the first call
+
+
+def _bind():
+    """The extension with the short way for plain forward calls; it answers None to what is not plain."""
+    global _fast
+    path = os.path.join(L.HERE, "csrc", "_fastcall.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    spec = importlib.util.spec_from_file_location("_fastcall", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    lib = L.lib()
+    mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in ("b200_add_rms_norm", "b200_linear_act", "b200_gated_linear", "b200_linear_act_q8",
+                                                                                "b200_linear_act_q8_workspace_bytes", "b200_error_string")})
+    _fast = mod
+    return mod
 
 
 def _call(name: str, index: int, *args) -> None:
@@ -221,6 +245,9 @@ class _AddRmsNorm(torch.autograd.Function):
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """x, residual [..., D] bf16 | fp16 | fp32 -> (y, s): s = x + residual (x itself without a residual), y = s / sqrt(mean(s^2) + eps) * weight.
     The norm is taken of the unrounded fp32 sum.  weight [D] in x's type or fp32, or None for ones.  Differentiable."""
+    plain = (_fast or _bind()).norm(x, residual, weight, eps, False, True)
+    if plain is not None:
+        return plain
     index, D = _norm_args(x, residual, weight, eps)
     if _wants_grad(x, residual, weight):
         out = _AddRmsNorm.apply(x, residual, weight, float(eps))
@@ -235,6 +262,9 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None = None, we
     """The same norm with y in 8 bits -> (q8, sf, s[, y]): q8 uint8 e4m3 codes [rows, D], sf uint8 E8M0 [rows, D/32], rows = all leading
     dimensions together (what `cukern.mx_grouped` and `linear_act_q8` take); q8 * 2^(sf - 127) is y quantised per 32 from its fp32 value.  want_y:
     y in x's type too.  D % 32 == 0.  No gradient."""
+    plain = (_fast or _bind()).norm(x, residual, weight, eps, True, want_y)
+    if plain is not None:
+        return plain
     index, D = _norm_args(x, residual, weight, eps)
     assert D % 32 == 0, f"width {D} is not a multiple of 32"
     assert not _wants_grad(x, residual, weight), "add_rms_norm_quant has no gradient: use add_rms_norm, or detach its inputs"
@@ -319,6 +349,9 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     (z Phi(z)) or "gelu_tanh".  fp32 accumulation, one rounding at the end.  Any K, N and number of rows; rows of x or w that do not start on
     16 bytes (a K that is no multiple of 8, an odd slice) are copied first.  Differentiable in x, w, bias and residual; with an activation a call
     that needs a gradient also keeps the pre-activation (N fp32 values per row)."""
+    out = (_fast or _bind()).linear(x, w, bias, _ACT.get(act, -1), residual)
+    if out is not None:
+        return out
     index, code, dt = _device(x, w, bias, residual), _act_code(act), x.dtype
     assert dt in _PAIR and w.dtype is dt and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
     (N, K), xs = w.shape, x.shape
@@ -338,6 +371,9 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
     """The projection on FP8 operands: x8 uint8 e4m3 [rows, K] + xsf uint8 E8M0 [rows, K/32] (`add_rms_norm_quant`, `cukern.mx_quantize_rows`), w8
     uint8 e4m3 [N, K] in natural k order (`w8.unpermute_k` of a W8's bytes) + s8 uint8 E8M0 [ceil(N/32), K/32].  bias [N], residual [rows, N] and
     the result bf16; products and sums in fp32.  K % 128 == 0.  No gradient."""
+    out = (_fast or _bind()).q8(x8, xsf, w8, s8, bias, _ACT.get(act, -1), residual)
+    if out is not None:
+        return out
     index, code, u8 = _device(x8, xsf, w8, s8, bias, residual), _act_code(act), torch.uint8
     assert x8.dtype is u8 and xsf.dtype is u8 and w8.dtype is u8 and s8.dtype is u8, "x8, xsf, w8 and s8 are uint8"
     assert x8.dim() == 2 and w8.dim() == 2 and xsf.dim() == 2 and s8.dim() == 2, "x8, xsf, w8 and s8 are matrices"
@@ -408,6 +444,9 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", l
     """act(min(g, limit)) * min(max(u, -limit), limit) with [g | u] = x w13^T, both projections and the product in one kernel: x [..., K], w13
     [2 * inter, K] (gate rows, then up rows: the layout of the expert weights), both bf16 or both fp16 -> [..., inter].  limit 0: no clamps.
     Differentiable in x and w13; a call that needs a gradient also keeps g and u (2 * inter fp32 values per row)."""
+    out = (_fast or _bind()).gated(x, w13, _ACT.get(act, -1), limit)
+    if out is not None:
+        return out
     index, code, dt = _device(x, w13), _act_code(act), x.dtype
     assert dt in _PAIR and w13.dtype is dt and w13.dim() == 2, "x and w13 must be both bfloat16 or both float16, w13 [2 * inter, K]"
     (n2, K), xs = w13.shape, x.shape
