@@ -1,11 +1,14 @@
-// Short way from Python to the forward calls of the dense operators.  A one-token call is bound by the host: through ctypes and torch's Python it takes
-// 10 to 14 us, of which the launch is 3; from here 5 to 8.  Each function takes the plain case only (CUDA tensors of one device, the current one;
-// contiguous, fetchable rows; no gradient wanted; shapes and types that fit) and answers None to everything else, which dense.py then checks, refuses or
-// lays out.  The kernels are the same entry points of libb200moe.so; their addresses are handed in once by dense.py.
+// Short way from Python to the calls of the dense operators.  A one-token call is bound by the host: through ctypes and torch's Python it takes 10 to
+// 14 us, of which the launch is 3; from here 4 to 6.  A training step of one small projection takes 132 us with autograd functions in Python and 76
+// with the ones here (torch's own linear: 98).  Each function takes the plain case only (CUDA tensors of one device, the current one; contiguous, fetchable
+// rows; shapes and types that fit) and answers None to everything else, which dense.py then checks, refuses or lays out.  The kernels are the same
+// entry points of libb200moe.so; their addresses are handed in once by dense.py.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <map>
@@ -24,6 +27,12 @@ int (*f_linear)(const void*, long long, const void*, long long, int, int, int, i
 int (*f_gated)(const void*, long long, const void*, long long, int, int, int, int, int, float, void*, long long, float*, long long, void*) = nullptr;
 int (*f_q8)(const void*, const void*, const void*, const void*, int, int, int, int, const void*, int, const void*, long long, void*, long long, void*, size_t, void*) = nullptr;
 size_t (*f_q8_ws)(int, int, int) = nullptr;
+size_t (*f_norm_bwd_ws)(long long, int) = nullptr;
+int (*f_norm_bwd)(const void*, long long, const void*, long long, const void*, int, int, long long, int, float, const void*, const void*, void*, void*, void*, size_t, void*) = nullptr;
+size_t (*f_linear_bwd_ws)(int, int) = nullptr;
+int (*f_linear_bwd)(const void*, long long, const float*, long long, int, int, int, int, void*, long long, void*, void*, size_t, void*) = nullptr;
+int (*f_gated_bwd)(const void*, long long, const float*, long long, int, float, int, int, int, void*, long long, void*) = nullptr;
+int (*f_product)(const void*, long long, int, const void*, long long, int, int, int, int, int, void*, long long, void*) = nullptr;
 const char* (*f_error)(int) = nullptr;
 
 void bind(const std::map<std::string, uintptr_t>& a) {
@@ -32,6 +41,12 @@ void bind(const std::map<std::string, uintptr_t>& a) {
     f_gated = reinterpret_cast<decltype(f_gated)>(a.at("b200_gated_linear"));
     f_q8 = reinterpret_cast<decltype(f_q8)>(a.at("b200_linear_act_q8"));
     f_q8_ws = reinterpret_cast<decltype(f_q8_ws)>(a.at("b200_linear_act_q8_workspace_bytes"));
+    f_norm_bwd_ws = reinterpret_cast<decltype(f_norm_bwd_ws)>(a.at("b200_add_rms_norm_bwd_workspace_bytes"));
+    f_norm_bwd = reinterpret_cast<decltype(f_norm_bwd)>(a.at("b200_add_rms_norm_bwd"));
+    f_linear_bwd_ws = reinterpret_cast<decltype(f_linear_bwd_ws)>(a.at("b200_linear_act_bwd_workspace_bytes"));
+    f_linear_bwd = reinterpret_cast<decltype(f_linear_bwd)>(a.at("b200_linear_act_bwd"));
+    f_gated_bwd = reinterpret_cast<decltype(f_gated_bwd)>(a.at("b200_gated_linear_bwd"));
+    f_product = reinterpret_cast<decltype(f_product)>(a.at("b200_dense_product"));
     f_error = reinterpret_cast<decltype(f_error)>(a.at("b200_error_string"));
 }
 
@@ -39,10 +54,12 @@ void check(int rc, const char* what) {
     if (rc) throw std::runtime_error(std::string(what) + " failed with CUDA error " + std::to_string(rc) + " (" + f_error(rc) + ")");
 }
 
-// contiguous, on the given device, of the given type, no gradient wanted
-bool plain(const Tensor& t, int dev, at::ScalarType type) {
-    return t.is_cuda() && t.get_device() == dev && t.scalar_type() == type && t.is_contiguous() && !(t.requires_grad() && c10::GradMode::is_enabled());
-}
+// contiguous, on the given device, of the given type
+bool plain(const Tensor& t, int dev, at::ScalarType type) { return t.is_cuda() && t.get_device() == dev && t.scalar_type() == type && t.is_contiguous(); }
+bool wants(const Tensor& t) { return t.requires_grad(); }
+bool wants(const OptTensor& t) { return t && t->requires_grad(); }
+template <typename... Ts>
+bool wants_grad(const Ts&... ts) { return c10::GradMode::is_enabled() && (... || wants(ts)); }
 bool fits16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 void* stream(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
@@ -73,28 +90,178 @@ Tensor like_rows(const Tensor& x, int64_t width) {
     return at::empty(shape, x.options().requires_grad(false));
 }
 
+// ------------------------------------------------------------------ launches
+void launch_norm(const Tensor& x, const OptTensor& res, const OptTensor& w, double eps, const Tensor& y, const Tensor& s, const Tensor& q8, const Tensor& sf) {
+    const int dev = x.get_device();
+    const int64_t D = x.size(-1);
+    auto p = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check(f_norm(x.data_ptr(), D, ptr(res), D, ptr(w), w && w->scalar_type() == at::kFloat, x.scalar_type() == at::kFloat ? 2 : half_type(x), x.numel() / D, (int)D, (float)eps, p(y),
+                 p(s), p(q8), p(sf), stream(dev)),
+          "b200_add_rms_norm");
+}
+void launch_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, int act, const OptTensor& res, const Tensor& out, float* z) {
+    const int64_t N = w.size(0), K = w.size(1);
+    check(f_linear(x.data_ptr(), K, w.data_ptr(), K, half_type(x), (int)(x.numel() / K), (int)N, (int)K, ptr(bias), act, ptr(res), N, out.data_ptr(), N, z, N, stream(x.get_device())),
+          "b200_linear_act");
+}
+void launch_gated(const Tensor& x, const Tensor& w13, int act, double limit, const Tensor& out, float* gu) {
+    const int64_t n2 = w13.size(0), K = w13.size(1);
+    check(f_gated(x.data_ptr(), K, w13.data_ptr(), K, half_type(x), (int)(x.numel() / K), (int)(n2 / 2), (int)K, act, (float)limit, out.data_ptr(), n2 / 2, gu, n2,
+                  stream(x.get_device())),
+          "b200_gated_linear");
+}
+// [M, N] = A B^T over K, dense operands (rows of A: K values, or M with a_mn; rows of B: N values)
+Tensor product(const Tensor& a, int a_mn, const Tensor& b, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape) {
+    Tensor out = at::empty(shape, b.options().requires_grad(false));
+    check(f_product(a.data_ptr(), a_mn ? M : K, a_mn, b.data_ptr(), N, 1, half_type(b), (int)M, (int)N, (int)K, out.data_ptr(), N, stream(b.get_device())), "b200_dense_product");
+    return out;
+}
+
+// ------------------------------------------------------------------ gradients
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// as torch's once_differentiable: gradients of gradients that want one raise when they are asked for
+variable_list once(variable_list out, const variable_list& grads) {
+    bool again = false;
+    for (const Tensor& g : grads) again = again || (g.defined() && g.requires_grad());
+    if (!again || !c10::GradMode::is_enabled()) return out;
+    auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int)out.size());
+    variable_list in;
+    for (const Tensor& t : out) {
+        in.push_back(t.defined() ? t.detach() : t);
+        if (t.defined()) in.back().requires_grad_(true);
+    }
+    return (*error)(std::move(in));
+}
+// incoming gradients as dense rows the kernels can fetch
+Tensor dense(const Tensor& g) {
+    Tensor d = g.contiguous();
+    return fits16(d) ? d : d.clone();
+}
+
+struct NormFn : torch::autograd::Function<NormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& res, const OptTensor& w, double eps) {
+        const auto opt = x.options().requires_grad(false);
+        Tensor y = at::empty(x.sizes(), opt), s;
+        if (res) s = at::empty(x.sizes(), opt);
+        launch_norm(x, res, w, eps, y, s, Tensor(), Tensor());
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({x, res ? *res : Tensor(), w ? *w : Tensor()});
+        ctx->saved_data["eps"] = eps;
+        return res ? variable_list{y, s} : variable_list{y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &r = saved[1], &w = saved[2];
+        const bool need_x = ctx->needs_input_grad(0), need_r = r.defined() && ctx->needs_input_grad(1), need_w = w.defined() && ctx->needs_input_grad(r.defined() ? 2 : 1);
+        const Tensor gs_in = grads.size() > 1 ? grads[1] : Tensor();
+        if (!grads[0].defined())  // the normed output was not used
+            return once({need_x ? gs_in : Tensor(), need_r ? gs_in : Tensor(), need_w ? at::zeros_like(w) : Tensor(), Tensor()}, grads);
+        const Tensor gy = dense(grads[0]), gs = gs_in.defined() ? dense(gs_in) : gs_in;
+        const int64_t D = x.size(-1), rows = x.numel() / D;
+        const size_t nb = need_w ? f_norm_bwd_ws(rows, (int)D) : 0;
+        Tensor ds = at::empty(x.sizes(), x.options().requires_grad(false)), dw, ws;
+        if (need_w) {
+            dw = at::empty(w.sizes(), w.options().requires_grad(false));
+            ws = at::empty({(int64_t)nb}, x.options().dtype(at::kByte).requires_grad(false));
+        }
+        check(f_norm_bwd(x.data_ptr(), D, r.defined() ? r.data_ptr() : nullptr, D, w.defined() ? w.data_ptr() : nullptr, w.defined() && w.scalar_type() == at::kFloat,
+                         x.scalar_type() == at::kFloat ? 2 : half_type(x), rows, (int)D, (float)ctx->saved_data["eps"].toDouble(), gy.data_ptr(), gs.defined() ? gs.data_ptr() : nullptr,
+                         ds.data_ptr(), need_w ? dw.data_ptr() : nullptr, need_w ? ws.data_ptr() : nullptr, nb, stream(x.get_device())),
+              "b200_add_rms_norm_bwd");
+        return once({need_x ? ds : Tensor(), need_r ? ds : Tensor(), dw, Tensor()}, grads);
+    }
+};
+
+struct LinearFn : torch::autograd::Function<LinearFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& res, int64_t act) {
+        Tensor out = like_rows(x, w.size(0)), z;
+        if (act) z = at::empty({x.numel() / w.size(1), w.size(0)}, x.options().dtype(at::kFloat).requires_grad(false));
+        launch_linear(x, w, bias, (int)act, res, out, act ? z.data_ptr<float>() : nullptr);
+        ctx->save_for_backward({x, w, z});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->saved_data["res"] = res.has_value();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &z = saved[2];
+        const int act = (int)ctx->saved_data["act"].toInt();
+        const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["res"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2),
+                   need_r = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+        const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
+        const Tensor gy = dense(grads[0]);
+        Tensor dz = gy, db, ws, dx, dw;
+        const auto opt = x.options().requires_grad(false);
+        if (act && (need_x || need_w)) dz = at::empty({M, N}, opt);
+        if (need_b) db = at::empty({N}, opt);
+        const bool own_dz = act && (need_x || need_w);
+        if (own_dz || need_b) {
+            const size_t nb = need_b ? f_linear_bwd_ws((int)M, (int)N) : 0;
+            if (nb) ws = at::empty({(int64_t)nb}, opt.dtype(at::kByte));
+            check(f_linear_bwd(gy.data_ptr(), N, act ? z.data_ptr<float>() : nullptr, N, act, half_type(x), (int)M, (int)N, own_dz ? dz.data_ptr() : nullptr, N,
+                               need_b ? db.data_ptr() : nullptr, nb ? ws.data_ptr() : nullptr, nb, stream(x.get_device())),
+                  "b200_linear_act_bwd");
+        }
+        if (need_x) dx = product(dz, 0, w, M, K, N, x.sizes());
+        if (need_w) dw = product(dz, 1, x, N, K, M, w.sizes());
+        return once({dx, dw, db, need_r ? grads[0] : Tensor(), Tensor()}, grads);
+    }
+};
+
+struct GatedFn : torch::autograd::Function<GatedFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w13, int64_t act, double limit) {
+        const int64_t n2 = w13.size(0);
+        Tensor out = like_rows(x, n2 / 2), gu = at::empty({x.numel() / w13.size(1), n2}, x.options().dtype(at::kFloat).requires_grad(false));
+        launch_gated(x, w13, (int)act, limit, out, gu.data_ptr<float>());
+        ctx->save_for_backward({x, w13, gu});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["limit"] = limit;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &gu = saved[2];
+        const int64_t n2 = w.size(0), K = w.size(1), M = x.numel() / K;
+        const Tensor gy = dense(grads[0]);
+        Tensor dgu = at::empty({M, n2}, x.options().requires_grad(false)), dx, dw;
+        check(f_gated_bwd(gy.data_ptr(), n2 / 2, gu.data_ptr<float>(), n2, (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["limit"].toDouble(), half_type(x), (int)M,
+                          (int)(n2 / 2), dgu.data_ptr(), n2, stream(x.get_device())),
+              "b200_gated_linear_bwd");
+        if (ctx->needs_input_grad(0)) dx = product(dgu, 0, w, M, K, n2, x.sizes());
+        if (ctx->needs_input_grad(1)) dw = product(dgu, 1, x, n2, K, M, w.sizes());
+        return once({dx, dw, Tensor(), Tensor()}, grads);
+    }
+};
+
+// ------------------------------------------------------------------ calls
 py::object norm(const Tensor& x, const OptTensor& res, const OptTensor& w, double eps, bool quant, bool want_y) {
     const int dev = plain_device(x);
     if (dev < 0) return py::none();
     const auto type = x.scalar_type();
     const int64_t D = x.size(-1);
-    const int code = type == at::kFloat ? 2 : half_type(x);
-    if (code < 0 || D > 16384 || !(eps >= 0) || !plain(x, dev, type)) return py::none();
+    if ((type != at::kFloat && half_type(x) < 0) || D > 16384 || !(eps >= 0) || !plain(x, dev, type)) return py::none();
     if (res && (!plain(*res, dev, type) || !res->sizes().equals(x.sizes()))) return py::none();
     if (w && (w->dim() != 1 || w->size(0) != D || !(plain(*w, dev, type) || plain(*w, dev, at::kFloat)))) return py::none();
-    if (quant && D % 32) return py::none();
+    const auto opt = x.options().requires_grad(false);
+    if (wants_grad(x, res, w)) {
+        if (quant) return py::none();
+        variable_list out = NormFn::apply(x, res, w, eps);
+        return py::make_tuple(out[0], res ? out[1] : x);
+    }
     const int64_t rows = x.numel() / D;
     Tensor y, s, q8, sf;
-    const auto opt = x.options().requires_grad(false);
     if (want_y) y = at::empty(x.sizes(), opt);
     if (res) s = at::empty(x.sizes(), opt);
     if (quant) {
+        if (D % 32) return py::none();
         q8 = at::empty({rows, D}, opt.dtype(at::kByte));
         sf = at::empty({rows, D / 32}, opt.dtype(at::kByte));
     }
-    check(f_norm(x.data_ptr(), D, ptr(res), D, ptr(w), w && w->scalar_type() == at::kFloat, code, rows, (int)D, (float)eps, want_y ? y.data_ptr() : nullptr,
-                 res ? s.data_ptr() : nullptr, quant ? q8.data_ptr() : nullptr, quant ? sf.data_ptr() : nullptr, stream(dev)),
-          "b200_add_rms_norm");
+    launch_norm(x, res, w, eps, y, s, q8, sf);
     if (!res) s = x;
     if (!quant) return py::make_tuple(y, s);
     return want_y ? py::make_tuple(q8, sf, s, y) : py::make_tuple(q8, sf, s);
@@ -104,22 +271,21 @@ py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias, int a
     const int dev = plain_device(x);
     if (dev < 0 || act < 0 || !product_fits(x, w, dev)) return py::none();
     const auto type = x.scalar_type();
-    const int64_t N = w.size(0), K = w.size(1);
+    const int64_t N = w.size(0);
     if (bias && (bias->dim() != 1 || bias->size(0) != N || !plain(*bias, dev, type))) return py::none();
     if (res && (!plain(*res, dev, type) || !same_but_last(*res, x, N))) return py::none();
+    if (wants_grad(x, w, bias, res)) return N % 8 ? py::object(py::none()) : py::cast(Tensor(LinearFn::apply(x, w, bias, res, (int64_t)act)));
     Tensor out = like_rows(x, N);
-    check(f_linear(x.data_ptr(), K, w.data_ptr(), K, half_type(x), (int)(x.numel() / K), (int)N, (int)K, ptr(bias), act, ptr(res), N, out.data_ptr(), N, nullptr, 0, stream(dev)),
-          "b200_linear_act");
+    launch_linear(x, w, bias, act, res, out, nullptr);
     return py::cast(out);
 }
 
 py::object gated(const Tensor& x, const Tensor& w13, int act, double limit) {
     const int dev = plain_device(x);
     if (dev < 0 || act < 0 || !(limit >= 0) || !product_fits(x, w13, dev) || w13.size(0) % 2) return py::none();
-    const int64_t inter = w13.size(0) / 2, K = w13.size(1);
-    Tensor out = like_rows(x, inter);
-    check(f_gated(x.data_ptr(), K, w13.data_ptr(), K, half_type(x), (int)(x.numel() / K), (int)inter, (int)K, act, (float)limit, out.data_ptr(), inter, nullptr, 0, stream(dev)),
-          "b200_gated_linear");
+    if (wants_grad(x, w13)) return w13.size(0) % 8 ? py::object(py::none()) : py::cast(Tensor(GatedFn::apply(x, w13, (int64_t)act, limit)));
+    Tensor out = like_rows(x, w13.size(0) / 2);
+    launch_gated(x, w13, act, limit, out, nullptr);
     return py::cast(out);
 }
 
@@ -132,6 +298,7 @@ py::object q8(const Tensor& x8, const Tensor& xsf, const Tensor& w8, const Tenso
     if (K % 128 || w8.size(1) != K || N < 1 || xsf.size(0) != M || xsf.size(1) != K / 32 || s8.size(0) != (N + 31) / 32 || s8.size(1) < K / 32) return py::none();
     if (!fits16(x8) || !fits16(w8) || (reinterpret_cast<uintptr_t>(xsf.data_ptr()) & 3) || M > INT32_MAX || N > (1 << 30) || K > (1 << 30) || s8.size(1) > INT32_MAX) return py::none();
     if (bias && (bias->dim() != 1 || bias->size(0) != N || !plain(*bias, dev, at::kBFloat16))) return py::none();
+    if (wants_grad(bias, res)) return py::none();
     if (res && (!plain(*res, dev, at::kBFloat16) || res->dim() != 2 || res->size(0) != M || res->size(1) != N)) return py::none();
     Tensor out = at::empty({M, N}, x8.options().dtype(at::kBFloat16)), ws;
     const size_t nb = f_q8_ws((int)M, (int)N, (int)K);

@@ -34,7 +34,7 @@ _fast = None  # csrc/fastcall.cpp, bound on the first call
 
 
 def _bind():
-    """The extension with the short way for plain forward calls; it answers None to what is not plain."""
+    """The extension with the short way for plain calls; it answers None to what is not plain."""
     global _fast
     path = os.path.join(L.HERE, "csrc", "_fastcall.so")
     if not os.path.exists(path):
@@ -43,8 +43,9 @@ def _bind():
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     lib = L.lib()
-    mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in ("b200_add_rms_norm", "b200_linear_act", "b200_gated_linear", "b200_linear_act_q8",
-                                                                                "b200_linear_act_q8_workspace_bytes", "b200_error_string")})
+    mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+        "b200_add_rms_norm", "b200_add_rms_norm_bwd_workspace_bytes", "b200_add_rms_norm_bwd", "b200_linear_act", "b200_linear_act_bwd_workspace_bytes", "b200_linear_act_bwd",
+        "b200_gated_linear", "b200_gated_linear_bwd", "b200_dense_product", "b200_linear_act_q8", "b200_linear_act_q8_workspace_bytes", "b200_error_string")})
     _fast = mod
     return mod
 

@@ -654,3 +654,41 @@ def test_no_second_derivatives(D, dev):
         assert all(torch.equal(a, b) for a, b in zip(plain, graph))
         with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
             torch.autograd.grad(graph[0].float().sum(), leaves[1])
+
+
+@pytest.mark.parametrize("n", [64, 50])  # 50: rows that the kernels cannot fetch, another way through the host code
+def test_gradients_of_some_inputs(D, dev, n):
+    """Whatever subset of the inputs wants a gradient, each gets the one of the full call."""
+    t, k, m = torch.bfloat16, 72, 19
+    vals = {"x": randn((m, k), 1, dev, t), "w": randn((n, k), 2, dev, t, 0.1), "bias": randn((n,), 3, dev, t), "residual": randn((m, n), 4, dev, t)}
+    gy = randn((m, n), 5, dev, t)
+    full = {a: v.clone().requires_grad_(True) for a, v in vals.items()}
+    ref = dict(zip(full, torch.autograd.grad(D.linear_act(act="gelu", **full), list(full.values()), gy)))
+    for names in (("x",), ("w",), ("bias",), ("residual",), ("x", "residual"), ("w", "bias"), ("bias", "residual")):
+        for drop in (None, "bias", "residual"):
+            if drop in names:
+                continue
+            args = {a: v.clone().requires_grad_(a in names) for a, v in vals.items() if a != drop}
+            got = torch.autograd.grad(D.linear_act(act="gelu", **args), [args[a] for a in names], gy)
+            for a, g in zip(names, got):
+                if drop != "bias":  # without the bias the slopes are others
+                    assert torch.equal(g, ref[a]), (names, drop, a)
+                assert g.shape == vals[a].shape and g.isfinite().all()
+    w13 = randn((2 * n, k), 6, dev, t, 0.1)
+    xg, wg = vals["x"].clone().requires_grad_(True), w13.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(D.gated_linear(xg, wg, limit=2.0), (xg, wg), gy)
+    assert torch.equal(torch.autograd.grad(D.gated_linear(xg, w13, limit=2.0), xg, gy)[0], dx)
+    assert torch.equal(torch.autograd.grad(D.gated_linear(vals["x"], wg, limit=2.0), wg, gy)[0], dw)
+    nw, r = randn((k,), 7, dev, t), randn((m, k), 8, dev, t)
+    gk = randn((m, k), 9, dev, t)
+    P = [v.clone().requires_grad_(True) for v in (vals["x"], r, nw)]
+    ref3 = torch.autograd.grad(D.add_rms_norm(*P)[0], P, gk)
+    for mask in range(1, 8):
+        Q = [v.clone().requires_grad_(bool(mask >> i & 1)) for i, v in enumerate((vals["x"], r, nw))]
+        want = [i for i in range(3) if mask >> i & 1]
+        got = torch.autograd.grad(D.add_rms_norm(*Q)[0], [Q[i] for i in want], gk)
+        assert all(torch.equal(g, ref3[i]) for g, i in zip(got, want))
+    q = nw.clone().requires_grad_(True)
+    full2 = torch.autograd.grad(D.add_rms_norm(vals["x"], None, q)[0], q, gk)[0]
+    x2 = vals["x"].clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(D.add_rms_norm(x2, None, q)[0], (x2, q), gk)[1], full2)
