@@ -1,7 +1,7 @@
 // Short way from Python to the calls of the dense operators.  A one-token call is bound by the host: through ctypes and torch's Python it takes 10 to
 // 14 us, of which the launch is 3; from here 4 to 6.  A training step of one small projection takes 132 us with autograd functions in Python and 76
-// with the ones here (torch's own linear: 98).  Each function takes the plain case only (CUDA tensors of one device, the current one; contiguous, fetchable
-// rows; shapes and types that fit) and answers None to everything else, which dense.py then checks, refuses or lays out.  The kernels are the same
+// with the ones here (torch's own linear: 98).  Each function takes the plain case only (CUDA tensors of one device, the current one; contiguous;
+// shapes and types that fit) and answers None to everything else, which dense.py then checks, refuses or lays out.  The kernels are the same
 // entry points of libb200moe.so; their addresses are handed in once by dense.py.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -32,6 +32,7 @@ int (*f_norm_bwd)(const void*, long long, const void*, long long, const void*, i
 size_t (*f_linear_bwd_ws)(int, int) = nullptr;
 int (*f_linear_bwd)(const void*, long long, const float*, long long, int, int, int, int, void*, long long, void*, void*, size_t, void*) = nullptr;
 int (*f_gated_bwd)(const void*, long long, const float*, long long, int, float, int, int, int, void*, long long, void*) = nullptr;
+int (*f_align)(const void*, long long, void*, long long, const void*, long long, void*, long long, int, long long, void*) = nullptr;
 int (*f_product)(const void*, long long, int, const void*, long long, int, int, int, int, int, void*, long long, void*) = nullptr;
 const char* (*f_error)(int) = nullptr;
 
@@ -46,6 +47,7 @@ void bind(const std::map<std::string, uintptr_t>& a) {
     f_linear_bwd_ws = reinterpret_cast<decltype(f_linear_bwd_ws)>(a.at("b200_linear_act_bwd_workspace_bytes"));
     f_linear_bwd = reinterpret_cast<decltype(f_linear_bwd)>(a.at("b200_linear_act_bwd"));
     f_gated_bwd = reinterpret_cast<decltype(f_gated_bwd)>(a.at("b200_gated_linear_bwd"));
+    f_align = reinterpret_cast<decltype(f_align)>(a.at("b200_align_rows"));
     f_product = reinterpret_cast<decltype(f_product)>(a.at("b200_dense_product"));
     f_error = reinterpret_cast<decltype(f_error)>(a.at("b200_error_string"));
 }
@@ -76,7 +78,7 @@ int half_type(const Tensor& x) { return x.scalar_type() == at::kBFloat16 ? 0 : x
 bool product_fits(const Tensor& x, const Tensor& w, int dev) {
     if (w.dim() != 2 || half_type(x) < 0 || !plain(x, dev, x.scalar_type()) || !plain(w, dev, x.scalar_type())) return false;
     const int64_t K = w.size(1), rows = x.numel() / x.size(-1);
-    return x.size(-1) == K && K % 8 == 0 && w.size(0) > 0 && fits16(x) && fits16(w) && rows <= INT32_MAX && w.size(0) <= (1 << 30) && K <= (1 << 30);
+    return x.size(-1) == K && K > 0 && w.size(0) > 0 && rows <= (1 << 30) && w.size(0) <= (1 << 30) && K <= (1 << 30);
 }
 bool same_but_last(const Tensor& a, const Tensor& b, int64_t last) {
     if (a.dim() != b.dim() || a.size(-1) != last) return false;
@@ -90,6 +92,40 @@ Tensor like_rows(const Tensor& x, int64_t width) {
     return at::empty(shape, x.options().requires_grad(false));
 }
 
+int64_t pitch(int64_t n) { return (n + 7) / 8 * 8; }
+
+// x [.., K] and w [N, K] as the kernels fetch them: themselves, or one copy of both with rows that start on 16 bytes (x's rows, then w's)
+struct Operands {
+    Tensor copy;  // defined: holds both
+    const void *x, *w;
+    int64_t M, N, K, ld;
+};
+Operands operands(const Tensor& x, const Tensor& w) {
+    Operands o{Tensor(), x.data_ptr(), w.data_ptr(), x.numel() / w.size(1), w.size(0), w.size(1), w.size(1)};
+    if (o.K % 8 == 0 && fits16(x) && fits16(w)) return o;
+    o.ld = pitch(o.K);
+    o.copy = at::empty({o.M + o.N, o.ld}, x.options().requires_grad(false));
+    char* p = static_cast<char*>(o.copy.data_ptr());
+    check(f_align(o.x, o.K, p, o.M, o.w, o.K, p + 2 * o.M * o.ld, o.N, (int)o.K, o.ld, stream(x.get_device())), "b200_align_rows");
+    o.x = p;
+    o.w = p + 2 * o.M * o.ld;
+    return o;
+}
+// what a backward pass keeps of them, and the way back
+void keep(torch::autograd::AutogradContext* ctx, const Operands& o, const Tensor& x, const Tensor& w, const Tensor& z) {
+    if (o.copy.defined()) ctx->save_for_backward({o.copy, Tensor(), z});
+    else ctx->save_for_backward({x, w, z});
+    ctx->saved_data["M"] = o.M;
+    ctx->saved_data["N"] = o.N;
+    ctx->saved_data["K"] = o.K;
+}
+Operands kept(torch::autograd::AutogradContext* ctx, const std::vector<Tensor>& saved) {
+    Operands o{saved[1].defined() ? Tensor() : saved[0], saved[0].data_ptr(), nullptr, ctx->saved_data["M"].toInt(), ctx->saved_data["N"].toInt(), ctx->saved_data["K"].toInt(), 0};
+    o.ld = o.copy.defined() ? pitch(o.K) : o.K;
+    o.w = o.copy.defined() ? static_cast<const char*>(o.x) + 2 * o.M * o.ld : saved[1].data_ptr();
+    return o;
+}
+
 // ------------------------------------------------------------------ launches
 void launch_norm(const Tensor& x, const OptTensor& res, const OptTensor& w, double eps, const Tensor& y, const Tensor& s, const Tensor& q8, const Tensor& sf) {
     const int dev = x.get_device();
@@ -99,21 +135,18 @@ void launch_norm(const Tensor& x, const OptTensor& res, const OptTensor& w, doub
                  p(s), p(q8), p(sf), stream(dev)),
           "b200_add_rms_norm");
 }
-void launch_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, int act, const OptTensor& res, const Tensor& out, float* z) {
-    const int64_t N = w.size(0), K = w.size(1);
-    check(f_linear(x.data_ptr(), K, w.data_ptr(), K, half_type(x), (int)(x.numel() / K), (int)N, (int)K, ptr(bias), act, ptr(res), N, out.data_ptr(), N, z, N, stream(x.get_device())),
+void launch_linear(const Operands& o, const Tensor& like, const OptTensor& bias, int act, const OptTensor& res, const Tensor& out, float* z) {
+    check(f_linear(o.x, o.ld, o.w, o.ld, half_type(like), (int)o.M, (int)o.N, (int)o.K, ptr(bias), act, ptr(res), o.N, out.data_ptr(), o.N, z, pitch(o.N), stream(like.get_device())),
           "b200_linear_act");
 }
-void launch_gated(const Tensor& x, const Tensor& w13, int act, double limit, const Tensor& out, float* gu) {
-    const int64_t n2 = w13.size(0), K = w13.size(1);
-    check(f_gated(x.data_ptr(), K, w13.data_ptr(), K, half_type(x), (int)(x.numel() / K), (int)(n2 / 2), (int)K, act, (float)limit, out.data_ptr(), n2 / 2, gu, n2,
-                  stream(x.get_device())),
+void launch_gated(const Operands& o, const Tensor& like, int act, double limit, const Tensor& out, float* gu) {
+    check(f_gated(o.x, o.ld, o.w, o.ld, half_type(like), (int)o.M, (int)(o.N / 2), (int)o.K, act, (float)limit, out.data_ptr(), o.N / 2, gu, pitch(o.N), stream(like.get_device())),
           "b200_gated_linear");
 }
-// [M, N] = A B^T over K, dense operands (rows of A: K values, or M with a_mn; rows of B: N values)
-Tensor product(const Tensor& a, int a_mn, const Tensor& b, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape) {
-    Tensor out = at::empty(shape, b.options().requires_grad(false));
-    check(f_product(a.data_ptr(), a_mn ? M : K, a_mn, b.data_ptr(), N, 1, half_type(b), (int)M, (int)N, (int)K, out.data_ptr(), N, stream(b.get_device())), "b200_dense_product");
+// [M, N] = A B^T over K: element (i, k) of A at a[i * a_ld + k] or, with a_mn, a[k * a_ld + i]; of B at b[k * b_ld + i]
+Tensor product(const Tensor& like, const void* a, int64_t a_ld, int a_mn, const void* b, int64_t b_ld, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape) {
+    Tensor out = at::empty(shape, like.options().requires_grad(false));
+    check(f_product(a, a_ld, a_mn, b, b_ld, 1, half_type(like), (int)M, (int)N, (int)K, out.data_ptr(), N, stream(like.get_device())), "b200_dense_product");
     return out;
 }
 
@@ -176,10 +209,12 @@ struct NormFn : torch::autograd::Function<NormFn> {
 
 struct LinearFn : torch::autograd::Function<LinearFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& res, int64_t act) {
-        Tensor out = like_rows(x, w.size(0)), z;
-        if (act) z = at::empty({x.numel() / w.size(1), w.size(0)}, x.options().dtype(at::kFloat).requires_grad(false));
-        launch_linear(x, w, bias, (int)act, res, out, act ? z.data_ptr<float>() : nullptr);
-        ctx->save_for_backward({x, w, z});
+        const Operands o = operands(x, w);
+        Tensor out = like_rows(x, o.N), z;
+        if (act) z = at::empty({o.M, pitch(o.N)}, x.options().dtype(at::kFloat).requires_grad(false));
+        launch_linear(o, x, bias, (int)act, res, out, act ? z.data_ptr<float>() : nullptr);
+        keep(ctx, o, x, w, z);
+        ctx->saved_data["x"] = x.sizes().vec();
         ctx->saved_data["act"] = act;
         ctx->saved_data["bias"] = bias.has_value();
         ctx->saved_data["res"] = res.has_value();
@@ -187,52 +222,54 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &z = saved[2];
-        const int act = (int)ctx->saved_data["act"].toInt();
+        const Tensor &like = saved[0], &z = saved[2];
+        const Operands o = kept(ctx, saved);
+        const int act = (int)ctx->saved_data["act"].toInt(), dev = like.get_device();
         const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["res"].toBool();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2),
                    need_r = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
-        const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
         const Tensor gy = dense(grads[0]);
-        Tensor dz = gy, db, ws, dx, dw;
-        const auto opt = x.options().requires_grad(false);
-        if (act && (need_x || need_w)) dz = at::empty({M, N}, opt);
-        if (need_b) db = at::empty({N}, opt);
-        const bool own_dz = act && (need_x || need_w);
+        const auto opt = like.options().requires_grad(false);
+        const bool own_dz = (act || o.N % 8) && (need_x || need_w);
+        const int64_t dz_ld = own_dz ? pitch(o.N) : o.N;
+        Tensor dz = own_dz ? at::empty({o.M, dz_ld}, opt) : gy, db, ws, dx, dw;
+        if (need_b) db = at::empty({o.N}, opt);
         if (own_dz || need_b) {
-            const size_t nb = need_b ? f_linear_bwd_ws((int)M, (int)N) : 0;
+            const size_t nb = need_b ? f_linear_bwd_ws((int)o.M, (int)o.N) : 0;
             if (nb) ws = at::empty({(int64_t)nb}, opt.dtype(at::kByte));
-            check(f_linear_bwd(gy.data_ptr(), N, act ? z.data_ptr<float>() : nullptr, N, act, half_type(x), (int)M, (int)N, own_dz ? dz.data_ptr() : nullptr, N,
-                               need_b ? db.data_ptr() : nullptr, nb ? ws.data_ptr() : nullptr, nb, stream(x.get_device())),
+            check(f_linear_bwd(gy.data_ptr(), o.N, act ? z.data_ptr<float>() : nullptr, pitch(o.N), act, half_type(like), (int)o.M, (int)o.N, own_dz ? dz.data_ptr() : nullptr, dz_ld,
+                               need_b ? db.data_ptr() : nullptr, nb ? ws.data_ptr() : nullptr, nb, stream(dev)),
                   "b200_linear_act_bwd");
         }
-        if (need_x) dx = product(dz, 0, w, M, K, N, x.sizes());
-        if (need_w) dw = product(dz, 1, x, N, K, M, w.sizes());
+        if (need_x) dx = product(like, dz.data_ptr(), dz_ld, 0, o.w, o.ld, o.M, o.K, o.N, ctx->saved_data["x"].toIntVector());
+        if (need_w) dw = product(like, dz.data_ptr(), dz_ld, 1, o.x, o.ld, o.N, o.K, o.M, {o.N, o.K});
         return once({dx, dw, db, need_r ? grads[0] : Tensor(), Tensor()}, grads);
     }
 };
 
 struct GatedFn : torch::autograd::Function<GatedFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w13, int64_t act, double limit) {
-        const int64_t n2 = w13.size(0);
-        Tensor out = like_rows(x, n2 / 2), gu = at::empty({x.numel() / w13.size(1), n2}, x.options().dtype(at::kFloat).requires_grad(false));
-        launch_gated(x, w13, (int)act, limit, out, gu.data_ptr<float>());
-        ctx->save_for_backward({x, w13, gu});
+        const Operands o = operands(x, w13);
+        Tensor out = like_rows(x, o.N / 2), gu = at::empty({o.M, pitch(o.N)}, x.options().dtype(at::kFloat).requires_grad(false));
+        launch_gated(o, x, (int)act, limit, out, gu.data_ptr<float>());
+        keep(ctx, o, x, w13, gu);
+        ctx->saved_data["x"] = x.sizes().vec();
         ctx->saved_data["act"] = act;
         ctx->saved_data["limit"] = limit;
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &gu = saved[2];
-        const int64_t n2 = w.size(0), K = w.size(1), M = x.numel() / K;
+        const Tensor &like = saved[0], &gu = saved[2];
+        const Operands o = kept(ctx, saved);
         const Tensor gy = dense(grads[0]);
-        Tensor dgu = at::empty({M, n2}, x.options().requires_grad(false)), dx, dw;
-        check(f_gated_bwd(gy.data_ptr(), n2 / 2, gu.data_ptr<float>(), n2, (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["limit"].toDouble(), half_type(x), (int)M,
-                          (int)(n2 / 2), dgu.data_ptr(), n2, stream(x.get_device())),
+        const int64_t ld = pitch(o.N);
+        Tensor dgu = at::empty({o.M, ld}, like.options().requires_grad(false)), dx, dw;
+        check(f_gated_bwd(gy.data_ptr(), o.N / 2, gu.data_ptr<float>(), ld, (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["limit"].toDouble(), half_type(like), (int)o.M,
+                          (int)(o.N / 2), dgu.data_ptr(), ld, stream(like.get_device())),
               "b200_gated_linear_bwd");
-        if (ctx->needs_input_grad(0)) dx = product(dgu, 0, w, M, K, n2, x.sizes());
-        if (ctx->needs_input_grad(1)) dw = product(dgu, 1, x, n2, K, M, w.sizes());
+        if (ctx->needs_input_grad(0)) dx = product(like, dgu.data_ptr(), ld, 0, o.w, o.ld, o.M, o.K, o.N, ctx->saved_data["x"].toIntVector());
+        if (ctx->needs_input_grad(1)) dw = product(like, dgu.data_ptr(), ld, 1, o.x, o.ld, o.N, o.K, o.M, {o.N, o.K});
         return once({dx, dw, Tensor(), Tensor()}, grads);
     }
 };
@@ -274,18 +311,18 @@ py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias, int a
     const int64_t N = w.size(0);
     if (bias && (bias->dim() != 1 || bias->size(0) != N || !plain(*bias, dev, type))) return py::none();
     if (res && (!plain(*res, dev, type) || !same_but_last(*res, x, N))) return py::none();
-    if (wants_grad(x, w, bias, res)) return N % 8 ? py::object(py::none()) : py::cast(Tensor(LinearFn::apply(x, w, bias, res, (int64_t)act)));
+    if (wants_grad(x, w, bias, res)) return py::cast(Tensor(LinearFn::apply(x, w, bias, res, (int64_t)act)));
     Tensor out = like_rows(x, N);
-    launch_linear(x, w, bias, act, res, out, nullptr);
+    launch_linear(operands(x, w), x, bias, act, res, out, nullptr);
     return py::cast(out);
 }
 
 py::object gated(const Tensor& x, const Tensor& w13, int act, double limit) {
     const int dev = plain_device(x);
     if (dev < 0 || act < 0 || !(limit >= 0) || !product_fits(x, w13, dev) || w13.size(0) % 2) return py::none();
-    if (wants_grad(x, w13)) return w13.size(0) % 8 ? py::object(py::none()) : py::cast(Tensor(GatedFn::apply(x, w13, (int64_t)act, limit)));
+    if (wants_grad(x, w13)) return py::cast(Tensor(GatedFn::apply(x, w13, (int64_t)act, limit)));
     Tensor out = like_rows(x, w13.size(0) / 2);
-    launch_gated(x, w13, act, limit, out, nullptr);
+    launch_gated(operands(x, w13), x, act, limit, out, nullptr);
     return py::cast(out);
 }
 

@@ -45,7 +45,7 @@ def _bind():
     lib = L.lib()
     mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
         "b200_add_rms_norm", "b200_add_rms_norm_bwd_workspace_bytes", "b200_add_rms_norm_bwd", "b200_linear_act", "b200_linear_act_bwd_workspace_bytes", "b200_linear_act_bwd",
-        "b200_gated_linear", "b200_gated_linear_bwd", "b200_dense_product", "b200_linear_act_q8", "b200_linear_act_q8_workspace_bytes", "b200_error_string")})
+        "b200_gated_linear", "b200_gated_linear_bwd", "b200_dense_product", "b200_align_rows", "b200_linear_act_q8", "b200_linear_act_q8_workspace_bytes", "b200_error_string")})
     _fast = mod
     return mod
 
