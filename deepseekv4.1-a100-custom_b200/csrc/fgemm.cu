@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
     }
     tc_fence_before();
     __syncwarp();
-    if constexpr (CG == 2 || SPLIT) cluster_sync();  // no CTA leaves while another may still signal its barriers or read its shared memory
+    if constexpr (CG == 2) cluster_sync();  // neither CTA of a pair leaves while the other may still signal its barriers or read its tensor memory
     else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
