@@ -276,44 +276,72 @@ __device__ __forceinline__ void epilogue_turned(const FgParams& P, float* buf, i
         buf[lane * FG_TURN_LD + 16 + i] = __uint_as_float(b[i]);
     }
     __syncwarp();
+    // Reads of the buffer and of the residual go ahead of the stores in groups: the compiler must assume that they alias (one row at a time, a turn of 32
+    // rows took 4 us).
     if (g.dual) {
-        const int col = col0 + (lane & 15);
+        const int c = lane & 15, col = col0 + c;
         if (col >= g.inter) return;
-#pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-            const int r = 2 * i + (lane >> 4);
-            const long long row = row0 + r;
-            float z = buf[r * FG_TURN_LD + (lane & 15)], u = buf[r * FG_TURN_LD + 16 + (lane & 15)];
-            if (row >= g.M) continue;
+#pragma unroll 1
+        for (int r0 = lane >> 4; r0 < 32; r0 += 16) {
+            float z[8], u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                z[i] = buf[(r0 + 2 * i) * FG_TURN_LD + c];
+                u[i] = buf[(r0 + 2 * i) * FG_TURN_LD + 16 + c];
+            }
+            const int rows = g.M - row0 - r0 < 16 ? (int)(g.M - row0 - r0) : 16;  // rows r0, r0 + 2, .. that exist: those with 2 i < rows
             if (g.z_out) {
-                g.z_out[row * g.z_ld + col] = z;
-                g.z_out[row * g.z_ld + g.inter + col] = u;
+                float* p = g.z_out + (row0 + r0) * g.z_ld + col;
+#pragma unroll
+                for (int i = 0; i < 8; ++i, p += 2 * g.z_ld)
+                    if (2 * i < rows) {
+                        p[0] = z[i];
+                        p[g.inter] = u[i];
+                    }
             }
             if (g.limit > 0.f) {
-                z = z > g.limit ? g.limit : z;
-                u = u > g.limit ? g.limit : (u < -g.limit ? -g.limit : u);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    z[i] = z[i] > g.limit ? g.limit : z[i];
+                    u[i] = u[i] > g.limit ? g.limit : (u[i] < -g.limit ? -g.limit : u[i]);
+                }
             }
-            reinterpret_cast<T*>(g.out)[row * g.out_ld + col] = from_f32<T>(act_fwd(g.act, z) * u);
+            act_fwd_n(g.act, z);
+            T* o = reinterpret_cast<T*>(g.out) + (row0 + r0) * g.out_ld + col;
+#pragma unroll
+            for (int i = 0; i < 8; ++i, o += 2 * g.out_ld)
+                if (2 * i < rows) *o = from_f32<T>(z[i] * u[i]);
         }
     } else {
         const int col = col0 + lane;
         if (lane >= cols || col >= g.N) return;
         const float bias = g.bias ? to_f32(reinterpret_cast<const T*>(g.bias)[col]) : 0.f;
-        const T* res = reinterpret_cast<const T*>(g.res);
         const int rows = g.M - row0 < 32 ? (int)(g.M - row0) : 32;
-        for (int r0 = 0; r0 < rows; r0 += 8) {
-            float rv[8];
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 16) {
+            float z[16];
+            T rv[16];
+            if (g.res) {  // without a branch per row: rows behind the last one read its value
+                const T* p = reinterpret_cast<const T*>(g.res) + row0 * g.res_ld + col;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) rv[i] = res && r0 + i < rows ? to_f32(res[(row0 + r0 + i) * g.res_ld + col]) : 0.f;  // in flight together
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = r0 + i;
-                if (r >= rows) break;
-                float z = buf[r * FG_TURN_LD + lane] + bias;
-                if (g.z_out) g.z_out[(row0 + r) * g.z_ld + col] = z;
-                z = act_fwd(g.act, z) + rv[i];
-                reinterpret_cast<T*>(g.out)[(row0 + r) * g.out_ld + col] = from_f32<T>(z);
+                for (int i = 0; i < 16; ++i) rv[i] = p[min(r0 + i, rows - 1) * g.res_ld];
             }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z[i] = buf[(r0 + i) * FG_TURN_LD + lane] + bias;
+            if (g.z_out) {
+                float* p = g.z_out + (row0 + r0) * g.z_ld + col;
+#pragma unroll
+                for (int i = 0; i < 16; ++i, p += g.z_ld)
+                    if (r0 + i < rows) *p = z[i];
+            }
+            act_fwd_n(g.act, z);
+            if (g.res)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] += to_f32(rv[i]);
+            T* o = reinterpret_cast<T*>(g.out) + (row0 + r0) * g.out_ld + col;
+#pragma unroll
+            for (int i = 0; i < 16; ++i, o += g.out_ld)
+                if (r0 + i < rows) *o = from_f32<T>(z[i]);
         }
     }
 }
