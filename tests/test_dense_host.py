@@ -114,7 +114,8 @@ def test_c_boundary_refusals(mods):
     assert q8(p, p, p, p, 2, 2, 8, 64, n, 0, n, 0, p, 8, p, 1 << 30, n) == BAD_SHAPE
     assert q8(p, p, p, p, 3, 2, 8, 128, n, 0, n, 0, p, 8, p, 1 << 30, n) == BAD_SHAPE
     assert q8(odd, p, p, p, 4, 2, 8, 128, n, 0, n, 0, p, 8, p, 1 << 30, n) == BAD_ALIGN
-    need = lib.b200_linear_act_q8_workspace_bytes(2, 8, 128)
-    if need:
-        assert q8(p, p, p, p, 4, 2, 8, 128, n, 0, n, 0, p, 8, p, need - 1, n) == WORKSPACE
+    assert lib.b200_linear_act_q8_workspace_bytes(2, 8, 128) == 0  # decode-sized calls need none
+    need = lib.b200_linear_act_q8_workspace_bytes(32, 8, 128)
+    assert need > 0 and q8(p, p, p, p, 4, 32, 8, 128, n, 0, n, 0, p, 8, p, need - 1, n) == WORKSPACE
+    assert q8(p, p, p, p, 4, 32, 8, 128, n, 0, n, 0, p, 8, n, need, n) == WORKSPACE
     assert b"shape" in lib.b200_error_string(BAD_SHAPE) or lib.b200_error_string(BAD_SHAPE)
