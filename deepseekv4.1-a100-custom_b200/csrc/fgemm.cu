@@ -549,10 +549,15 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
         const int q = warp & 3, half = warp >= 8 ? 1 : 0, r = q * 32 + lane;
         const uint32_t t0 = tmem + ((uint32_t)(q * 32) << 16);
         auto column = [&](int owner, int j) { return g.dual ? (j < n2 ? owner * W2 + 16 * j : BN / 2 + owner * W2 + 16 * (j - n2)) : owner * W + 16 * j; };
+        const Tile t = tile_at(first, P.m_tiles, P.n_tiles);
+        const long long row = (long long)(t.m * CG + (int)rank) * FG_BM + r;
+        const bool some = warp >= 4 && row - lane < g.M;  // rows behind the last one are neither sent nor added
+        Ahead h;
+        if (some && !g.dual && !P.turned) fetch16(P, row, t.n * BN + slice * W + 16 * half, h);  // under the exchange
         __syncwarp();
         cluster_sync();  // every CTA's MMAs have read their stages
         tc_fence_after();
-        if (warp >= 4) {
+        if (some) {
             for (int o = 0; o < split; ++o) {
                 if (o == slice) continue;
                 const uint32_t dst = map_rank(smem_u32(ring), (uint32_t)(o * CG) + rank) + (uint32_t)(slice * (W / 4) * FG_BM + r) * 16u;
@@ -568,13 +573,9 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const FgParams P
                 }
             }
         }
-        const Tile t = tile_at(first, P.m_tiles, P.n_tiles);
-        const long long row = (long long)(t.m * CG + (int)rank) * FG_BM + r;
-        Ahead h;
-        if (warp >= 4 && !g.dual && !P.turned) fetch16(P, row, t.n * BN + slice * W + 16 * half, h);  // under the exchange
         __syncwarp();
         cluster_sync();
-        if (warp >= 4) {
+        if (some) {
             auto sum16 = [&](int j, uint32_t (&out)[16]) {
                 uint32_t a[16];
                 tc_ld16(t0 + column(slice, j), a);

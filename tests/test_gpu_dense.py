@@ -364,17 +364,29 @@ def test_linear_special_values(D, dev):
         assert v[0] == 1600.0 and v[1] == 0.0, (act, v)
 
 
-def test_linear_long_rows(D, dev):
-    """Many rows, a few columns: row offsets of the residual and the output pass 2^31 bytes (rows * 2 * stride)."""
-    m, ld = 70000, 16384
+def test_offsets_past_32_bits(D, dev):
+    """Rows whose element offsets pass 2^31, in x, the residual, the norm's inputs and the weights."""
+    m, ld = 140000, 16384
     buf = torch.empty(m, ld, device=dev, dtype=torch.bfloat16)
-    r = buf[:, 16000:16008]
+    r, xs = buf[:, 16000:16008], buf[:, 8000:8064]
     r.copy_(randn((m, 8), 1, dev, torch.bfloat16))
     x, w = randn((m, 64), 2, dev, torch.bfloat16), randn((8, 64), 3, dev, torch.bfloat16, 0.1)
     assert torch.equal(D.linear_act(x, w, None, None, r), D.linear_act(x, w, None, None, r.contiguous()))
-    xs = buf[:, 8000:8064]
     xs.copy_(x)
     assert torch.equal(D.linear_act(xs, w), D.linear_act(x, w))
+    assert torch.equal(D.add_rms_norm(xs, xs)[0], D.add_rms_norm(x, x)[0])
+    xg, xsg = x.clone().requires_grad_(True), xs.detach().requires_grad_(True)
+    gy = randn((m, 64), 4, dev, torch.bfloat16)
+    assert torch.equal(torch.autograd.grad(D.add_rms_norm(xg)[0], xg, gy)[0], torch.autograd.grad(D.add_rms_norm(xsg)[0], xsg, gy)[0])
+    del buf, r, xs, xsg
+    n, k = 600000, 4096
+    big = torch.empty(n, k, device=dev, dtype=torch.bfloat16)
+    rows = torch.tensor([0, 1, 31, 300000, 524288, 524289, 599998, 599999], device=dev)
+    big[rows] = randn((8, k), 5, dev, torch.bfloat16, 1 / 64)
+    for m in (2, 12, 40):  # streaming kernel, streaming kernel with two groups of rows, tensor cores
+        x = randn((m, k), 6, dev, torch.bfloat16)
+        ref, bound, _, _ = linear_bounds(x, big[rows], None, None, None, torch.bfloat16)
+        within(D.linear_act(x, big)[:, rows], ref, bound, f"m {m}")
 
 
 # ------------------------------------------------------------------ gated projection
