@@ -7,8 +7,8 @@
 // x is read at its use: after the first tile of an SM it is in L1, which the weights bypass.  The warps' partial sums meet in shared memory in warp
 // order (the same result from run to run).  The legacy mma.sync is enough here: at full HBM rate an SM issues one per 11 ns.
 //
-// Measured (graph replay, weights from HBM): 1 x 4096 x 2048 4.8 us, 8 x 4096 x 4096 8.5, 8 x 12288 x 4096 19.1 (5.3 TB/s); FP8 8 x 4096 x 4096 7.2,
-// 8 x 12288 x 4096 15.9.  What bounds it: a block's life (load, multiply, add up, store) is about 5 us of latencies, and an SM holds two or three;
+// Measured (graph replay, weights from HBM, with bias and residual): 1 x 4096 x 2048 5.2 us, 8 x 4096 x 4096 9.1, 8 x 12288 x 4096 20.0 (5.0 TB/s); FP8
+// 8 x 4096 x 4096 7.3, 8 x 12288 x 4096 17.1.  What bounds it: a block's life (load, multiply, add up, store) is about 5 us of latencies, and an SM holds two or three;
 // blocks that walk several tiles with the next loads in flight were slower (22.1 and 17.1 us for the 12288 rows: fewer warps fit).
 #include "fgemm.cuh"
 

@@ -659,7 +659,9 @@ def test_no_second_derivatives(D, dev):
     """Gradients with create_graph are the same values and refuse to be differentiated again."""
     x, w = randn((8, 64), 1, dev, torch.bfloat16).requires_grad_(True), randn((16, 64), 2, dev, torch.bfloat16).requires_grad_(True)
     n, w13 = randn((64,), 3, dev, torch.bfloat16).requires_grad_(True), randn((32, 64), 4, dev, torch.bfloat16).requires_grad_(True)
-    for f, leaves in ((lambda: D.linear_act(x, w, None, "gelu"), (x, w)), (lambda: D.gated_linear(x, w13), (x, w13)), (lambda: D.add_rms_norm(x, None, n)[0], (x, n))):
+    xs = randn((8, 80), 5, dev, torch.bfloat16)[:, 3:67].requires_grad_(True)  # rows that take the other way through the host code
+    for f, leaves in ((lambda: D.linear_act(x, w, None, "gelu"), (x, w)), (lambda: D.gated_linear(x, w13), (x, w13)), (lambda: D.add_rms_norm(x, None, n)[0], (x, n)),
+                      (lambda: D.linear_act(xs, w, None, "gelu"), (xs, w)), (lambda: D.gated_linear(xs, w13), (xs, w13)), (lambda: D.add_rms_norm(xs, None, n)[0], (xs, n))):
         y = f()
         plain = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
         graph = torch.autograd.grad(y, leaves, torch.ones_like(y), create_graph=True)
