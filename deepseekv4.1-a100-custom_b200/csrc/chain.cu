@@ -1163,7 +1163,7 @@ extern "C" int b200_device_error(int* code, cudaStream_t stream) {
     if ((rc = fg_device_error(&fg))) return rc;
     if ((rc = norm_device_error(&nm))) return rc;
     // prefill tensor-core kernel 11..41, streaming kernels 1001..1091, decode weight-stream kernel 2011..2042, messaging waits 3001..3004,
-    // 16-bit / FP8 GEMMs of the dense operators 4001..4021, norm backward 5001
+    // 16-bit / FP8 GEMMs of the dense operators 4001..4021, norm 5001 (backward), 5002 (forward)
     *code = mx ? mx : (sk ? 1000 + sk : (wm ? 2000 + wm : (pp ? 3000 + pp : (fg ? 4000 + fg : (nm ? 5000 + nm : 0)))));
     return 0;
 }
