@@ -96,12 +96,13 @@ int64_t pitch(int64_t n) { return (n + 7) / 8 * 8; }
 
 // x [.., K] and w [N, K] as the kernels fetch them: themselves, or one copy of both with rows that start on 16 bytes (x's rows, then w's)
 struct Operands {
-    Tensor copy;  // defined: holds both
+    Tensor copy;     // defined: holds both
+    Tensor kx, kw;   // of a backward pass: keep the memory of x and w where the copy does not
     const void *x, *w;
     int64_t M, N, K, ld;
 };
 Operands operands(const Tensor& x, const Tensor& w) {
-    Operands o{Tensor(), x.data_ptr(), w.data_ptr(), x.numel() / w.size(1), w.size(0), w.size(1), w.size(1)};
+    Operands o{Tensor(), Tensor(), Tensor(), x.data_ptr(), w.data_ptr(), x.numel() / w.size(1), w.size(0), w.size(1), w.size(1)};
     if (o.K % 8 == 0 && fits16(x) && fits16(w)) return o;
     o.ld = pitch(o.K);
     o.copy = at::empty({o.M + o.N, o.ld}, x.options().requires_grad(false));
@@ -119,10 +120,31 @@ void keep(torch::autograd::AutogradContext* ctx, const Operands& o, const Tensor
     ctx->saved_data["N"] = o.N;
     ctx->saved_data["K"] = o.K;
 }
-Operands kept(torch::autograd::AutogradContext* ctx, const std::vector<Tensor>& saved) {
-    Operands o{saved[1].defined() ? Tensor() : saved[0], saved[0].data_ptr(), nullptr, ctx->saved_data["M"].toInt(), ctx->saved_data["N"].toInt(), ctx->saved_data["K"].toInt(), 0};
-    o.ld = o.copy.defined() ? pitch(o.K) : o.K;
-    o.w = o.copy.defined() ? static_cast<const char*>(o.x) + 2 * o.M * o.ld : saved[1].data_ptr();
+// A saved tensor as the backward pass gets it.  A saved-tensor hook (save_on_cpu) may hand back other strides and another address than were saved: laid out
+// again here; not other sizes, type or device.
+Tensor restored(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, int dev) {
+    if (!t.defined() || !t.is_cuda() || t.get_device() != dev || t.scalar_type() != type || !t.sizes().equals(sizes))
+        throw std::runtime_error("a saved-tensor hook returned a tensor of other sizes, type or device than it was given");
+    Tensor d = t.contiguous();
+    return fits16(d) ? d : d.clone();
+}
+Operands kept(torch::autograd::AutogradContext* ctx, const std::vector<Tensor>& saved, at::ScalarType type, int dev) {
+    Operands o{};
+    o.M = ctx->saved_data["M"].toInt();
+    o.N = ctx->saved_data["N"].toInt();
+    o.K = ctx->saved_data["K"].toInt();
+    if (saved[1].defined()) {
+        o.ld = o.K;
+        o.kx = restored(saved[0], ctx->saved_data["x"].toIntVector(), type, dev);
+        o.kw = restored(saved[1], {o.N, o.K}, type, dev);
+        o.x = o.kx.data_ptr();
+        o.w = o.kw.data_ptr();
+    } else {
+        o.ld = pitch(o.K);
+        o.copy = restored(saved[0], {o.M + o.N, o.ld}, type, dev);
+        o.x = o.copy.data_ptr();
+        o.w = static_cast<const char*>(o.x) + 2 * o.M * o.ld;
+    }
     return o;
 }
 
@@ -182,16 +204,21 @@ struct NormFn : torch::autograd::Function<NormFn> {
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, res ? *res : Tensor(), w ? *w : Tensor()});
         ctx->saved_data["eps"] = eps;
+        ctx->saved_data["w_f32"] = w && w->scalar_type() == at::kFloat;
         return res ? variable_list{y, s} : variable_list{y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &r = saved[1], &w = saved[2];
+        Tensor x = saved[0], r = saved[1], w = saved[2];
         const bool need_x = ctx->needs_input_grad(0), need_r = r.defined() && ctx->needs_input_grad(1), need_w = w.defined() && ctx->needs_input_grad(r.defined() ? 2 : 1);
         const Tensor gs_in = grads.size() > 1 ? grads[1] : Tensor();
         if (!grads[0].defined())  // the normed output was not used
             return once({need_x ? gs_in : Tensor(), need_r ? gs_in : Tensor(), need_w ? at::zeros_like(w) : Tensor(), Tensor()}, grads);
         const Tensor gy = dense(grads[0]), gs = gs_in.defined() ? dense(gs_in) : gs_in;
+        const int dev = gy.get_device();
+        x = restored(x, gy.sizes(), gy.scalar_type(), dev);
+        if (r.defined()) r = restored(r, gy.sizes(), gy.scalar_type(), dev);
+        if (w.defined()) w = restored(w, {gy.size(-1)}, ctx->saved_data["w_f32"].toBool() ? at::kFloat : gy.scalar_type(), dev);
         const int64_t D = x.size(-1), rows = x.numel() / D;
         const size_t nb = need_w ? f_norm_bwd_ws(rows, (int)D) : 0;
         Tensor ds = at::empty(x.sizes(), x.options().requires_grad(false)), dw, ws;
@@ -222,13 +249,13 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &like = saved[0], &z = saved[2];
-        const Operands o = kept(ctx, saved);
-        const int act = (int)ctx->saved_data["act"].toInt(), dev = like.get_device();
+        const Tensor gy = dense(grads[0]), &like = gy;
+        const int act = (int)ctx->saved_data["act"].toInt(), dev = gy.get_device();
+        const Operands o = kept(ctx, saved, gy.scalar_type(), dev);
+        const Tensor z = act ? restored(saved[2], {o.M, pitch(o.N)}, at::kFloat, dev) : Tensor();
         const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["res"].toBool();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2),
                    need_r = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
-        const Tensor gy = dense(grads[0]);
         const auto opt = like.options().requires_grad(false);
         const bool own_dz = (act || o.N % 8) && (need_x || need_w);
         const int64_t dz_ld = own_dz ? pitch(o.N) : o.N;
@@ -260,13 +287,14 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &like = saved[0], &gu = saved[2];
-        const Operands o = kept(ctx, saved);
-        const Tensor gy = dense(grads[0]);
+        const Tensor gy = dense(grads[0]), &like = gy;
+        const int dev = gy.get_device();
+        const Operands o = kept(ctx, saved, gy.scalar_type(), dev);
         const int64_t ld = pitch(o.N);
+        const Tensor gu = restored(saved[2], {o.M, ld}, at::kFloat, dev);
         Tensor dgu = at::empty({o.M, ld}, like.options().requires_grad(false)), dx, dw;
         check(f_gated_bwd(gy.data_ptr(), o.N / 2, gu.data_ptr<float>(), ld, (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["limit"].toDouble(), half_type(like), (int)o.M,
-                          (int)(o.N / 2), dgu.data_ptr(), ld, stream(like.get_device())),
+                          (int)(o.N / 2), dgu.data_ptr(), ld, stream(dev)),
               "b200_gated_linear_bwd");
         if (ctx->needs_input_grad(0)) dx = product(like, dgu.data_ptr(), ld, 0, o.w, o.ld, o.M, o.K, o.N, ctx->saved_data["x"].toIntVector());
         if (ctx->needs_input_grad(1)) dw = product(like, dgu.data_ptr(), ld, 1, o.x, o.ld, o.N, o.K, o.M, {o.N, o.K});

@@ -184,6 +184,14 @@ def _scratch(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _restored(t: torch.Tensor, shape, dtype, device) -> torch.Tensor:
+    """A tensor as `ctx.saved_tensors` returns it.  A saved-tensor hook (`torch.autograd.graph.save_on_cpu`) may hand back other strides and another address
+    than were saved, so a backward pass takes both from here; other values' sizes, type or device it may not hand back."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise RuntimeError(f"a saved-tensor hook returned {t.dtype} {tuple(t.shape)} on {t.device} for {dtype} {tuple(shape)} on {device}")
+    return t
+
+
 # ------------------------------------------------------------------ residual addition + rms norm
 def _norm_args(x, residual, weight, eps):
     index, dt, D = _device(x, residual, weight), x.dtype, x.shape[-1]
@@ -215,7 +223,7 @@ class _AddRmsNorm(torch.autograd.Function):
         _norm_forward(x.get_device(), x.shape[-1], x2, r2, wc, eps, y, s, None, None)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x2, r2, wc)
-        ctx.eps, ctx.shape = eps, x.shape
+        ctx.eps, ctx.shape, ctx.rows, ctx.w_dtype = eps, x.shape, x2.shape, wc.dtype if wc is not None else None
         return (y, s) if residual is not None else y
 
     @staticmethod
@@ -230,7 +238,10 @@ class _AddRmsNorm(torch.autograd.Function):
         need_x, need_r, need_w, _ = ctx.needs_input_grad
         if gy is None:  # the normed output was not used
             return gs if need_x else None, gs if need_r else None, torch.zeros_like(w) if need_w else None, None
-        dev = x.device
+        dev = gy.device
+        x = _rows(_restored(x, ctx.rows, gy.dtype, dev))
+        r = _rows(_restored(r, ctx.rows, gy.dtype, dev)) if r is not None else None
+        w = _restored(w, (ctx.rows[1],), ctx.w_dtype, dev).contiguous() if w is not None else None
         gy = gy.contiguous()
         gs = gs.contiguous() if gs is not None else None
         rows, D = x.shape
@@ -303,7 +314,7 @@ class _LinearAct(torch.autograd.Function):
         z = torch.empty(M, z_ld, device=x.device, dtype=torch.float32) if act else None
         _linear_forward(x.get_device(), x.dtype, ops, M, N, K, bias, act, residual, out, z, z_ld)
         ctx.save_for_backward(ops[0], ops[3], z)
-        ctx.dims, ctx.lds, ctx.act, ctx.x_shape = (M, N, K), (ops[2], ops[5]), act, x.shape
+        ctx.dims, ctx.saved_shapes, ctx.act, ctx.x_shape = (M, N, K), (ops[0].shape, ops[3].shape), act, x.shape
         return out
 
     @staticmethod
@@ -316,7 +327,10 @@ class _LinearAct(torch.autograd.Function):
     def gradients(ctx, gy):
         x, w, z = ctx.saved_tensors
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
-        (M, N, K), (x_ld, w_ld), dev, dt = ctx.dims, ctx.lds, x.device, x.dtype
+        (M, N, K), dev, dt = ctx.dims, gy.device, gy.dtype
+        x, x_ld = _tma_rows(_restored(x, ctx.saved_shapes[0], dt, dev))
+        w, w_ld = _tma_rows(_restored(w, ctx.saved_shapes[1], dt, dev))
+        z = _restored(z, (M, _pitch(N)), torch.float32, dev).contiguous() if z is not None else None
         g2 = _rows(gy)
         dx = dw = db = None
         if need_b:
@@ -415,7 +429,7 @@ class _GatedLinear(torch.autograd.Function):
         gu = torch.empty(M, gu_ld, device=x.device, dtype=torch.float32)
         _gated_forward(x.get_device(), x.dtype, ops, M, inter, K, act, limit, out, gu, gu_ld)
         ctx.save_for_backward(ops[0], ops[3], gu)
-        ctx.dims, ctx.lds, ctx.act, ctx.limit, ctx.x_shape = (M, n2, K), (ops[2], ops[5]), act, limit, x.shape
+        ctx.dims, ctx.saved_shapes, ctx.act, ctx.limit, ctx.x_shape = (M, n2, K), (ops[0].shape, ops[3].shape), act, limit, x.shape
         return out
 
     @staticmethod
@@ -428,9 +442,12 @@ class _GatedLinear(torch.autograd.Function):
     def gradients(ctx, gy):
         x, w, gu = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        (M, n2, K), (x_ld, w_ld), dev, dt = ctx.dims, ctx.lds, x.device, x.dtype
-        g2 = _rows(gy)
+        (M, n2, K), dev, dt = ctx.dims, gy.device, gy.dtype
         gu_ld = _pitch(n2)
+        x, x_ld = _tma_rows(_restored(x, ctx.saved_shapes[0], dt, dev))
+        w, w_ld = _tma_rows(_restored(w, ctx.saved_shapes[1], dt, dev))
+        gu = _restored(gu, (M, gu_ld), torch.float32, dev).contiguous()
+        g2 = _rows(gy)
         dx = dw = None
         dgu = torch.empty(M, gu_ld, device=dev, dtype=dt)
         _call("b200_gated_linear_bwd", dev.index, g2.data_ptr(), _ld(g2), gu.data_ptr(), gu_ld, ctx.act, ctx.limit, _PAIR[dt], M, n2 // 2, dgu.data_ptr(), gu_ld)
