@@ -137,11 +137,15 @@ static int dense_check(int dtype, int act) {
     return act < ACT_NONE || act > ACT_GELU_TANH ? ERR_UNSUPPORTED : 0;
 }
 
+// rows and columns are counted in 32 bits, a tile's overhang included
+static bool too_large(int M, int N, int K) { return M > 1 << 30 || N > 1 << 30 || K > 1 << 30; }
+
 extern "C" int b200_linear_act(const void* x, long long x_ld, const void* w, long long w_ld, int dtype, int M, int N, int K, const void* bias, int act,
                                const void* residual, long long r_ld, void* out, long long out_ld, float* z, long long z_ld, cudaStream_t stream) {
     const int rc = dense_check(dtype, act);
     if (rc) return rc;
     if (M < 0 || N <= 0 || K <= 0) return ERR_BAD_SHAPE;
+    if (too_large(M, N, K)) return ERR_TOO_LARGE;
     if (M == 0) return 0;
     if (!x || !w || !out) return ERR_BAD_ARG;
     if (out_ld < N || (residual && r_ld < N) || (z && z_ld < N)) return ERR_BAD_SHAPE;
@@ -158,6 +162,7 @@ extern "C" int b200_gated_linear(const void* x, long long x_ld, const void* w13,
     const int rc = dense_check(dtype, act);
     if (rc) return rc;
     if (M < 0 || inter <= 0 || inter > (1 << 29) || K <= 0 || !(limit >= 0.f)) return ERR_BAD_SHAPE;
+    if (too_large(M, 2 * inter, K)) return ERR_TOO_LARGE;
     if (M == 0) return 0;
     if (!x || !w13 || !out) return ERR_BAD_ARG;
     if (out_ld < inter || (gu && gu_ld < 2 * inter)) return ERR_BAD_SHAPE;
@@ -174,6 +179,7 @@ extern "C" int b200_dense_product(const void* a_base, long long a_ld, int a_mn, 
     const int rc = dense_check(dtype, 0);
     if (rc) return rc;
     if (M < 0 || N < 0 || K <= 0 || out_ld < N) return ERR_BAD_SHAPE;
+    if (too_large(M, N, K)) return ERR_TOO_LARGE;
     if (M == 0 || N == 0) return 0;
     if (!a_base || !b_base || !out) return ERR_BAD_ARG;
     FgArgs a{};
@@ -194,6 +200,7 @@ extern "C" int b200_linear_act_bwd(const void* gy, long long gy_ld, const float*
     const int rc = dense_check(dtype, act);
     if (rc) return rc;
     if (M < 0 || N <= 0) return ERR_BAD_SHAPE;
+    if (too_large(M, N, 1)) return ERR_TOO_LARGE;
     if (act != ACT_NONE && M > 0 && !z) return ERR_BAD_ARG;
     if (M == 0) return dbias ? (int)cudaMemsetAsync(dbias, 0, (size_t)N * 2, stream) : 0;
     if (!gy || (!dz && !dbias)) return ERR_BAD_ARG;
@@ -213,6 +220,7 @@ extern "C" int b200_gated_linear_bwd(const void* gy, long long gy_ld, const floa
     const int rc = dense_check(dtype, act);
     if (rc) return rc;
     if (M < 0 || inter <= 0 || inter > (1 << 29) || !(limit >= 0.f)) return ERR_BAD_SHAPE;
+    if (too_large(M, 2 * inter, 1)) return ERR_TOO_LARGE;
     if (M == 0) return 0;
     if (!gy || !gu || !dgu) return ERR_BAD_ARG;
     if (gy_ld < inter || gu_ld < 2 * inter || dgu_ld < 2 * inter) return ERR_BAD_SHAPE;
@@ -241,6 +249,7 @@ extern "C" int b200_linear_act_q8(const void* x8, const void* xsf, const void* w
     const int rc = dense_check(F_BF16, act);
     if (rc) return rc;
     if (M < 0 || N <= 0 || K <= 0 || K % 128 || s_cols < K / 32) return ERR_BAD_SHAPE;
+    if (too_large(M, N, K)) return ERR_TOO_LARGE;
     if (M == 0) return 0;
     if (!x8 || !xsf || !w8 || !s8 || !out) return ERR_BAD_ARG;
     if (out_ld < N || (residual && r_ld < N)) return ERR_BAD_SHAPE;

@@ -361,7 +361,7 @@ py::object q8(const Tensor& x8, const Tensor& xsf, const Tensor& w8, const Tenso
         if (!plain(*t, dev, at::kByte)) return py::none();
     const int64_t M = x8.size(0), K = x8.size(1), N = w8.size(0);
     if (K % 128 || w8.size(1) != K || N < 1 || xsf.size(0) != M || xsf.size(1) != K / 32 || s8.size(0) != (N + 31) / 32 || s8.size(1) < K / 32) return py::none();
-    if (!fits16(x8) || !fits16(w8) || (reinterpret_cast<uintptr_t>(xsf.data_ptr()) & 3) || M > INT32_MAX || N > (1 << 30) || K > (1 << 30) || s8.size(1) > INT32_MAX) return py::none();
+    if (!fits16(x8) || !fits16(w8) || (reinterpret_cast<uintptr_t>(xsf.data_ptr()) & 3) || M > (1 << 30) || N > (1 << 30) || K > (1 << 30) || s8.size(1) > INT32_MAX) return py::none();
     if (bias && (bias->dim() != 1 || bias->size(0) != N || !plain(*bias, dev, at::kBFloat16))) return py::none();
     if (wants_grad(bias, res)) return py::none();
     if (res && (!plain(*res, dev, at::kBFloat16) || res->dim() != 2 || res->size(0) != M || res->size(1) != N)) return py::none();

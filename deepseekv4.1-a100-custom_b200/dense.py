@@ -353,6 +353,11 @@ class _LinearAct(torch.autograd.Function):
         return dx, dw, db, None, gy if need_r else None
 
 
+def _assert_counts(M: int, N: int, K: int) -> None:
+    """The library counts rows and columns in 32 bits, a tile's overhang included; ctypes would cut a larger number without a word."""
+    assert M <= 1 << 30 and N <= 1 << 30 and K <= 1 << 30, f"rows, N and K are 2^30 at most, got {M}, {N}, {K}"
+
+
 def _act_code(act) -> int:
     code = L.ACTIVATIONS.get(act)
     assert code is not None, f"act must be one of {sorted(a for a in L.ACTIVATIONS if a)} or None, got {act!r}"
@@ -361,7 +366,7 @@ def _act_code(act) -> int:
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
     """act(x w^T + bias) + residual: x [..., K], w [N, K], bias [N], residual [..., N], all bf16 or all fp16; act None, "relu", "silu", "gelu"
-    (z Phi(z)) or "gelu_tanh".  fp32 accumulation, one rounding at the end.  Any K, N and number of rows; rows of x or w that do not start on
+    (z Phi(z)) or "gelu_tanh".  fp32 accumulation, one rounding at the end.  Any K, N and number of rows up to 2^30; rows of x or w that do not start on
     16 bytes (a K that is no multiple of 8, an odd slice) are copied first.  Differentiable in x, w, bias and residual; with an activation a call
     that needs a gradient also keeps the pre-activation (N fp32 values per row)."""
     out = (_fast or _bind()).linear(x, w, bias, _ACT.get(act, -1), residual)
@@ -371,6 +376,7 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     assert dt in _PAIR and w.dtype is dt and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
     (N, K), xs = w.shape, x.shape
     assert xs and xs[-1] == K and K >= 1 and N >= 1, f"x {tuple(xs)} does not fit w {tuple(w.shape)}"
+    _assert_counts(x.numel() // K, N, K)
     shape = (*xs[:-1], N)
     assert bias is None or (bias.dtype is dt and bias.shape == (N,)), "bias must be [N] in x's type"
     assert residual is None or (residual.dtype is dt and residual.shape == shape), "residual must have the type and shape of the result"
@@ -394,7 +400,9 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
     assert x8.dim() == 2 and w8.dim() == 2 and xsf.dim() == 2 and s8.dim() == 2, "x8, xsf, w8 and s8 are matrices"
     (M, K), N = x8.shape, w8.shape[0]
     assert K % 128 == 0 and K > 0 and w8.shape[1] == K and N >= 1, f"x8 {tuple(x8.shape)} / w8 {tuple(w8.shape)}: the widths must be equal and a multiple of 128"
+    _assert_counts(M, N, K)
     s_rows, s_cols = s8.shape
+    assert s_cols < 1 << 31, f"s8 has {s_cols} columns"
     assert xsf.shape == (M, K // 32) and s_rows == (N + 31) // 32 and s_cols >= K // 32, "one scale per 32 k: xsf [rows, K/32], s8 [ceil(N/32), K/32]"
     assert bias is None or (bias.dtype is torch.bfloat16 and bias.shape == (N,)), "bias must be bfloat16 [N]"
     assert residual is None or (residual.dtype is torch.bfloat16 and residual.shape == (M, N)), "residual must be bfloat16 [rows, N]"
@@ -470,6 +478,7 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", l
     (n2, K), xs = w13.shape, x.shape
     assert n2 >= 2 and n2 % 2 == 0 and K >= 1 and xs and xs[-1] == K, f"x {tuple(xs)} does not fit w13 {tuple(w13.shape)}"
     assert limit >= 0.0, "limit must not be negative"
+    _assert_counts(x.numel() // K, n2, K)
     if _wants_grad(x, w13):
         return _GatedLinear.apply(x, w13, code, float(limit))
     out = torch.empty((*xs[:-1], n2 // 2), device=x.device, dtype=dt)

@@ -345,6 +345,7 @@ int b200_ep_close(void* ptr);
  * backward passes) and in FP8.  The reference computes these with torch (dsv41/model.py, Block and _swiglu :2337-2342); the clamps of the
  * gated product are those of dsv41/fused.py:291-296.
  * dtype: B200_BF16 / B200_FP16 (/ B200_FP32 for the norm); act: B200_ACT_*.  All sizes are element counts, *_ld are row strides in elements.
+ * M, N (2 inter) and K are 2^30 at most (B200_ERR_TOO_LARGE); the norm takes 2^31 - 1 rows.
  * Arguments are checked before anything is launched; M == 0 / rows == 0 is a valid call that writes nothing (weight and bias gradients: zeros).
  *
  * b200_add_rms_norm: s = x + residual (or x), y = s / sqrt(mean(s^2) + eps) * w (w NULL: 1), computed in fp32 from the unrounded sum; y and
