@@ -10,22 +10,24 @@ namespace b200 {
 
 // dz = gy * act'(z) and the column sums of dz.  z arrives in fp32: in 16 bits its rounding would put an error of the size of the result's own
 // rounding into every gradient.  8 warps of a block share DZ_ROWS rows of 32 * VEC columns; the sums of a block's rows go to
-// part[block row][N] in fp32 (from the unrounded dz), added in block order afterwards.  Bound by HBM: gy and z in, dz out.
+// part[row block][N] in fp32 (from the unrounded dz), added in block order afterwards.  Row and column blocks share grid x (y ends at 65535, which would
+// end the rows at 4.2 million).  Bound by HBM: gy and z in, dz out.
 constexpr int DZ_ROWS = 64;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const float* __restrict__ z, long long z_ld, int act, int M, int N,
-                                                      T* __restrict__ dz, long long dz_ld, float* __restrict__ part) {
+                                                      T* __restrict__ dz, long long dz_ld, float* __restrict__ part, int col_blocks) {
     __shared__ float red[8][32 * VEC];
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = (blockIdx.x * 32 + lane) * VEC;
-    const int r_end = min(M, (int)(blockIdx.y + 1) * DZ_ROWS);
+    const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
+    const int c = (cb * 32 + lane) * VEC;
+    const int r_end = min(M, (rb + 1) * DZ_ROWS);
     float sum[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
     if (c < N) {
-        for (int r = blockIdx.y * DZ_ROWS + warp; r < r_end; r += 8) {
+        for (int r = rb * DZ_ROWS + warp; r < r_end; r += 8) {
             float g[VEC];
             load_vec<T, VEC>(gy + r * gy_ld + c, g);
             if (z) {
@@ -48,8 +50,8 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, 
         float t = 0.f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) t += red[w][k];
-        const int col = (blockIdx.x * 32 + (k & 31)) * VEC + (k >> 5);
-        if (col < N) part[(long long)blockIdx.y * N + col] = t;
+        const int col = (cb * 32 + (k & 31)) * VEC + (k >> 5);
+        if (col < N) part[(long long)rb * N + col] = t;
     }
 }
 
@@ -112,10 +114,11 @@ static bool ok16(const void* p, long long ld) { return !((uintptr_t)p & 15) && l
 template <typename T>
 static int act_bwd_run(const void* gy, long long gy_ld, const float* z, long long z_ld, int act, int M, int N, void* dz, long long dz_ld, float* part, cudaStream_t stream) {
     const bool vec = N % 8 == 0 && ok16(gy, gy_ld) && (!z || ok16(z, z_ld)) && (!dz || ok16(dz, dz_ld));
-    const int w = vec ? 256 : 32;
-    const dim3 grid((N + w - 1) / w, (M + DZ_ROWS - 1) / DZ_ROWS);
-    return (int)launch_pdl(vec ? act_bwd_kernel<T, 8> : act_bwd_kernel<T, 1>, grid, dim3(256), 0, stream, (const T*)gy, gy_ld, z, z_ld, act, M, N, (T*)dz, dz_ld,
-                           part);
+    const int w = vec ? 256 : 32, col_blocks = (N + w - 1) / w;
+    const long long blocks = (long long)((M + DZ_ROWS - 1) / DZ_ROWS) * col_blocks;
+    if (blocks > 0x7FFFFFFFll) return ERR_TOO_LARGE;
+    return (int)launch_pdl(vec ? act_bwd_kernel<T, 8> : act_bwd_kernel<T, 1>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)gy, gy_ld, z, z_ld, act, M, N, (T*)dz,
+                           dz_ld, part, col_blocks);
 }
 
 template <typename T>
@@ -205,7 +208,6 @@ extern "C" int b200_linear_act_bwd(const void* gy, long long gy_ld, const float*
     if (M == 0) return dbias ? (int)cudaMemsetAsync(dbias, 0, (size_t)N * 2, stream) : 0;
     if (!gy || (!dz && !dbias)) return ERR_BAD_ARG;
     if (gy_ld < N || (z && z_ld < N) || (dz && dz_ld < N)) return ERR_BAD_SHAPE;
-    if ((M + DZ_ROWS - 1) / DZ_ROWS > 65535) return ERR_TOO_LARGE;
     if (dbias && (!workspace || workspace_bytes < b200_linear_act_bwd_workspace_bytes(M, N))) return ERR_WORKSPACE;
     float* part = dbias ? (float*)workspace : nullptr;
     if (act == ACT_NONE) z = nullptr;
