@@ -62,6 +62,11 @@ bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const OptTensor& t) { return t && t->requires_grad(); }
 template <typename... Ts>
 bool wants_grad(const Ts&... ts) { return c10::GradMode::is_enabled() && (... || wants(ts)); }
+// a forward-mode tangent: dense.py refuses the call
+bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool dual(const OptTensor& t) { return t && t->_fw_grad(0).defined(); }
+template <typename... Ts>
+bool any_dual(const Ts&... ts) { return (... || dual(ts)); }
 bool fits16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 void* stream(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
@@ -308,7 +313,7 @@ py::object norm(const Tensor& x, const OptTensor& res, const OptTensor& w, doubl
     if (dev < 0) return py::none();
     const auto type = x.scalar_type();
     const int64_t D = x.size(-1);
-    if ((type != at::kFloat && half_type(x) < 0) || D > 16384 || !(eps >= 0) || !plain(x, dev, type)) return py::none();
+    if ((type != at::kFloat && half_type(x) < 0) || D > 16384 || !(eps >= 0) || !plain(x, dev, type) || any_dual(x, res, w)) return py::none();
     if (res && (!plain(*res, dev, type) || !res->sizes().equals(x.sizes()))) return py::none();
     if (w && (w->dim() != 1 || w->size(0) != D || !(plain(*w, dev, type) || plain(*w, dev, at::kFloat)))) return py::none();
     const auto opt = x.options().requires_grad(false);
@@ -334,7 +339,7 @@ py::object norm(const Tensor& x, const OptTensor& res, const OptTensor& w, doubl
 
 py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias, int act, const OptTensor& res) {
     const int dev = plain_device(x);
-    if (dev < 0 || act < 0 || !product_fits(x, w, dev)) return py::none();
+    if (dev < 0 || act < 0 || !product_fits(x, w, dev) || any_dual(x, w, bias, res)) return py::none();
     const auto type = x.scalar_type();
     const int64_t N = w.size(0);
     if (bias && (bias->dim() != 1 || bias->size(0) != N || !plain(*bias, dev, type))) return py::none();
@@ -347,7 +352,7 @@ py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias, int a
 
 py::object gated(const Tensor& x, const Tensor& w13, int act, double limit) {
     const int dev = plain_device(x);
-    if (dev < 0 || act < 0 || !(limit >= 0) || !product_fits(x, w13, dev) || w13.size(0) % 2) return py::none();
+    if (dev < 0 || act < 0 || !(limit >= 0) || !product_fits(x, w13, dev) || w13.size(0) % 2 || any_dual(x, w13)) return py::none();
     if (wants_grad(x, w13)) return py::cast(Tensor(GatedFn::apply(x, w13, (int64_t)act, limit)));
     Tensor out = like_rows(x, w13.size(0) / 2);
     launch_gated(operands(x, w13), x, act, limit, out, nullptr);
@@ -363,7 +368,7 @@ py::object q8(const Tensor& x8, const Tensor& xsf, const Tensor& w8, const Tenso
     if (K % 128 || w8.size(1) != K || N < 1 || xsf.size(0) != M || xsf.size(1) != K / 32 || s8.size(0) != (N + 31) / 32 || s8.size(1) < K / 32) return py::none();
     if (!fits16(x8) || !fits16(w8) || (reinterpret_cast<uintptr_t>(xsf.data_ptr()) & 3) || M > (1 << 30) || N > (1 << 30) || K > (1 << 30) || s8.size(1) > INT32_MAX) return py::none();
     if (bias && (bias->dim() != 1 || bias->size(0) != N || !plain(*bias, dev, at::kBFloat16))) return py::none();
-    if (wants_grad(bias, res)) return py::none();
+    if (wants_grad(bias, res) || any_dual(bias, res)) return py::none();
     if (res && (!plain(*res, dev, at::kBFloat16) || res->dim() != 2 || res->size(0) != M || res->size(1) != N)) return py::none();
     Tensor out = at::empty({M, N}, x8.options().dtype(at::kBFloat16)), ws;
     const size_t nb = f_q8_ws((int)M, (int)N, (int)K);

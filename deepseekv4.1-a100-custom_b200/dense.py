@@ -4,8 +4,8 @@ bias, activation and residual in its epilogue (`linear_act`, `linear_act_q8`), t
 tensors' device; nothing synchronises.  Scratch and outputs come from torch's allocator per call, so calls on several streams, and captured
 CUDA graphs, share no memory.
 
-`add_rms_norm`, `linear_act` and `gated_linear` are differentiable (once); the FP8 forms are for serving and refuse inputs that require a
-gradient.  A captured backward pass needs what torch asks of any: capture it on the stream that ran the warm-up, and drop eager graphs of the
+`add_rms_norm`, `linear_act` and `gated_linear` are differentiable (once, in reverse mode; inputs with a forward-mode tangent are
+refused); the FP8 forms are for serving and refuse inputs that require a gradient.  A captured backward pass needs what torch asks of any: capture it on the stream that ran the warm-up, and drop eager graphs of the
 same leaves first."""
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import importlib.util
 import os
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -169,6 +170,12 @@ def _wants_grad(a, b=None, c=None, d=None) -> bool:
     return _grad_enabled() and (a.requires_grad or b is not None and b.requires_grad or c is not None and c.requires_grad or d is not None and d.requires_grad)
 
 
+def _no_tangents(*ts) -> None:
+    """Inputs that carry a forward-mode tangent are refused: the result would have none, which torch takes for a derivative of zero."""
+    if any(t is not None and unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("the dense operators have no forward-mode derivatives")
+
+
 def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K, shape=None) -> torch.Tensor:
     out = torch.empty(shape or (M, N), device=a.device, dtype=a.dtype)
     _call("b200_dense_product", a.get_device(), a.data_ptr(), a_ld, a_mn, b.data_ptr(), b_ld, b_mn, _PAIR[a.dtype], M, N, K, out.data_ptr(), N)
@@ -260,6 +267,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: 
     plain = (_fast or _bind()).norm(x, residual, weight, eps, False, True)
     if plain is not None:
         return plain
+    _no_tangents(x, residual, weight)
     index, D = _norm_args(x, residual, weight, eps)
     if _wants_grad(x, residual, weight):
         out = _AddRmsNorm.apply(x, residual, weight, float(eps))
@@ -277,6 +285,7 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None = None, we
     plain = (_fast or _bind()).norm(x, residual, weight, eps, True, want_y)
     if plain is not None:
         return plain
+    _no_tangents(x, residual, weight)
     index, D = _norm_args(x, residual, weight, eps)
     assert D % 32 == 0, f"width {D} is not a multiple of 32"
     assert not _wants_grad(x, residual, weight), "add_rms_norm_quant has no gradient: use add_rms_norm, or detach its inputs"
@@ -372,6 +381,7 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     out = (_fast or _bind()).linear(x, w, bias, _ACT.get(act, -1), residual)
     if out is not None:
         return out
+    _no_tangents(x, w, bias, residual)
     index, code, dt = _device(x, w, bias, residual), _act_code(act), x.dtype
     assert dt in _PAIR and w.dtype is dt and w.dim() == 2, "x and w must be both bfloat16 or both float16, w [N, K]"
     (N, K), xs = w.shape, x.shape
@@ -395,6 +405,7 @@ def linear_act_q8(x8: torch.Tensor, xsf: torch.Tensor, w8: torch.Tensor, s8: tor
     out = (_fast or _bind()).q8(x8, xsf, w8, s8, bias, _ACT.get(act, -1), residual)
     if out is not None:
         return out
+    _no_tangents(bias, residual)
     index, code, u8 = _device(x8, xsf, w8, s8, bias, residual), _act_code(act), torch.uint8
     assert x8.dtype is u8 and xsf.dtype is u8 and w8.dtype is u8 and s8.dtype is u8, "x8, xsf, w8 and s8 are uint8"
     assert x8.dim() == 2 and w8.dim() == 2 and xsf.dim() == 2 and s8.dim() == 2, "x8, xsf, w8 and s8 are matrices"
@@ -473,6 +484,7 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, act: str | None = "silu", l
     out = (_fast or _bind()).gated(x, w13, _ACT.get(act, -1), limit)
     if out is not None:
         return out
+    _no_tangents(x, w13)
     index, code, dt = _device(x, w13), _act_code(act), x.dtype
     assert dt in _PAIR and w13.dtype is dt and w13.dim() == 2, "x and w13 must be both bfloat16 or both float16, w13 [2 * inter, K]"
     (n2, K), xs = w13.shape, x.shape

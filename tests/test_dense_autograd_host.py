@@ -103,3 +103,24 @@ def test_another_tensor_from_a_hook_is_refused(D, monkeypatch, unpack):
     for f in (lambda: D._LinearAct.apply(x, w, None, 3, None), lambda: D._GatedLinear.apply(x, w, 2, 0.0), lambda: D._AddRmsNorm.apply(x, x, n, 1e-6)):
         with pytest.raises(RuntimeError, match="saved-tensor hook"):
             backward(f, Hooks(unpack))
+
+
+def test_forward_mode_is_refused(D, monkeypatch):
+    """A result without a tangent would count as one whose derivative is zero."""
+    import torch.autograd.forward_ad as fw
+    monkeypatch.setattr(D.L, "require_cuda", lambda *t: torch.device("cpu"))
+    rec = Recorder(D, monkeypatch)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8)  # noqa: E731
+    with fw.dual_level():
+        dual = lambda *s: fw.make_dual(bf(*s), bf(*s))  # noqa: E731
+        for call in (lambda: D.linear_act(dual(2, 64), bf(8, 64)), lambda: D.linear_act(bf(2, 64), dual(8, 64)), lambda: D.linear_act(bf(2, 64), bf(8, 64), dual(8)),
+                     lambda: D.linear_act(bf(2, 64), bf(8, 64), residual=dual(2, 8)), lambda: D.gated_linear(dual(2, 64), bf(8, 64)), lambda: D.gated_linear(bf(2, 64), dual(8, 64)),
+                     lambda: D.add_rms_norm(dual(2, 64)), lambda: D.add_rms_norm(bf(2, 64), dual(2, 64)), lambda: D.add_rms_norm(bf(2, 64), None, dual(64)),
+                     lambda: D.add_rms_norm_quant(dual(2, 64)), lambda: D.linear_act_q8(u8(2, 128), u8(2, 4), u8(8, 128), u8(1, 4), bias=dual(8)),
+                     lambda: D.linear_act_q8(u8(2, 128), u8(2, 4), u8(8, 128), u8(1, 4), residual=dual(2, 8))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert not rec.calls
+        D.linear_act(bf(2, 64), bf(8, 64))  # without tangents a level changes nothing
+        assert len(rec.calls) == 1

@@ -82,3 +82,29 @@ def test_other_tensors_from_hooks_are_refused(D, dev, kind, unpack):
             y = f()
         with pytest.raises(RuntimeError, match="saved-tensor hook"):
             torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("kind", ["dense", "odd"])
+def test_forward_mode_is_refused(D, dev, kind):
+    """Whichever input carries the tangent, with and without a gradient wanted or recorded."""
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        for grad in (False, True):
+            for recorded in (False, True):
+                for which in ("x", "w", "bias", "residual"):
+                    P = {a: t.detach().requires_grad_(grad) for a, t in operands(dev, kind).items()}
+                    n = randn((72,), 5, dev).requires_grad_(grad)
+                    P[which] = fw.make_dual(P[which], torch.ones_like(P[which]))
+                    with torch.set_grad_enabled(recorded):
+                        fs = [lambda: D.linear_act(P["x"], P["w"], P["bias"], "gelu", P["residual"])]
+                        if which in ("x", "w"):
+                            fs.append(lambda: D.gated_linear(P["x"], P["w"]))
+                        if which == "x":
+                            fs += [lambda: D.add_rms_norm(P["x"]), lambda: D.add_rms_norm(P["x"], None, n), lambda: D.add_rms_norm(P["x"].detach() * 0, P["x"]),
+                                   lambda: D.add_rms_norm_quant(torch.cat([P["x"]] * 4, 1))]
+                        for f in fs:
+                            with pytest.raises(NotImplementedError, match="forward-mode"):
+                                f()
+    x, w = randn((4, 64), 1, dev), randn((8, 64), 2, dev)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda a: D.linear_act(a, w), (x,), (torch.ones_like(x),))
