@@ -8,7 +8,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <map>
@@ -181,18 +183,27 @@ Tensor product(const Tensor& like, const void* a, int64_t a_ld, int a_mn, const 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// as torch's once_differentiable: gradients of gradients that want one raise when they are asked for
-variable_list once(variable_list out, const variable_list& grads) {
-    bool again = false;
-    for (const Tensor& g : grads) again = again || (g.defined() && g.requires_grad());
-    if (!again || !c10::GradMode::is_enabled()) return out;
-    auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int)out.size());
-    variable_list in;
-    for (const Tensor& t : out) {
-        in.push_back(t.defined() ? t.detach() : t);
-        if (t.defined()) in.back().requires_grad_(true);
+// The gradients of a backward pass that records its graph (create_graph).  They cannot be differentiated again; a node that raises when that is tried stands
+// behind each, with edges to what the gradient depends on: `inputs[i]`, positions among this function's tensor inputs, and the incoming gradients.  So it is
+// met on the way to any of these, whichever leaves are asked for and whether the incoming gradients are constants or not; a gradient that depends on
+// nothing that wants one stays a plain tensor.
+using Inputs = std::vector<int>;
+std::vector<Tensor> once(std::vector<Tensor> out, const std::vector<Inputs>& inputs, const std::vector<Tensor>& incoming) {
+    namespace ag = torch::autograd;
+    if (!c10::GradMode::is_enabled()) return out;
+    const auto self = ag::get_current_node();
+    for (size_t i = 0; i < out.size(); ++i) {
+        if (!out[i].defined() || !out[i].is_floating_point()) continue;
+        ag::edge_list edges;
+        for (int j : inputs[i])
+            if (j < (int)self->num_outputs() && self->next_edge(j).is_valid()) edges.push_back(self->next_edge(j));
+        for (const Tensor& g : incoming)
+            if (g.defined() && g.requires_grad()) edges.push_back(ag::impl::gradient_edge(g));
+        if (edges.empty()) continue;
+        out[i] = out[i].detach();
+        ag::set_history(out[i], std::make_shared<ag::Error>("trying to differentiate twice a function that was marked with @once_differentiable", std::move(edges)));
     }
-    return (*error)(std::move(in));
+    return out;
 }
 // incoming gradients as dense rows the kernels can fetch
 Tensor dense(const Tensor& g) {
@@ -218,7 +229,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
         const bool need_x = ctx->needs_input_grad(0), need_r = r.defined() && ctx->needs_input_grad(1), need_w = w.defined() && ctx->needs_input_grad(r.defined() ? 2 : 1);
         const Tensor gs_in = grads.size() > 1 ? grads[1] : Tensor();
         if (!grads[0].defined())  // the normed output was not used
-            return once({need_x ? gs_in : Tensor(), need_r ? gs_in : Tensor(), need_w ? at::zeros_like(w) : Tensor(), Tensor()}, grads);
+            return {need_x ? gs_in : Tensor(), need_r ? gs_in : Tensor(), need_w ? at::zeros(w.sizes(), w.options().requires_grad(false)) : Tensor(), Tensor()};
         const Tensor gy = dense(grads[0]), gs = gs_in.defined() ? dense(gs_in) : gs_in;
         const int dev = gy.get_device();
         x = restored(x, gy.sizes(), gy.scalar_type(), dev);
@@ -235,7 +246,11 @@ struct NormFn : torch::autograd::Function<NormFn> {
                          x.scalar_type() == at::kFloat ? 2 : half_type(x), rows, (int)D, (float)ctx->saved_data["eps"].toDouble(), gy.data_ptr(), gs.defined() ? gs.data_ptr() : nullptr,
                          ds.data_ptr(), need_w ? dw.data_ptr() : nullptr, need_w ? ws.data_ptr() : nullptr, nb, stream(x.get_device())),
               "b200_add_rms_norm_bwd");
-        return once({need_x ? ds : Tensor(), need_r ? ds : Tensor(), dw, Tensor()}, grads);
+        const bool has_r = r.defined(), has_w = w.defined();
+        const Inputs stream_in = has_r ? Inputs{0, 1} : Inputs{0};
+        Inputs all = stream_in;
+        if (has_w) all.push_back(has_r ? 2 : 1);
+        return once({need_x ? ds : Tensor(), need_r ? ds : Tensor(), dw, Tensor()}, {all, all, stream_in, {}}, grads);
     }
 };
 
@@ -275,7 +290,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         }
         if (need_x) dx = product(like, dz.data_ptr(), dz_ld, 0, o.w, o.ld, o.M, o.K, o.N, ctx->saved_data["x"].toIntVector());
         if (need_w) dw = product(like, dz.data_ptr(), dz_ld, 1, o.x, o.ld, o.N, o.K, o.M, {o.N, o.K});
-        return once({dx, dw, db, need_r ? grads[0] : Tensor(), Tensor()}, grads);
+        const bool curved = act > 1;  // without an activation, and with relu but for its corner, the slope does not depend on z
+        const Inputs of_z = curved ? (has_b ? Inputs{0, 1, 2} : Inputs{0, 1}) : Inputs{};
+        variable_list out = once({dx, dw, db}, {curved ? of_z : Inputs{1}, curved ? of_z : Inputs{0}, of_z}, grads);
+        return {out[0], out[1], out[2], need_r ? grads[0] : Tensor(), Tensor()};
     }
 };
 
@@ -303,7 +321,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
               "b200_gated_linear_bwd");
         if (ctx->needs_input_grad(0)) dx = product(like, dgu.data_ptr(), ld, 0, o.w, o.ld, o.M, o.K, o.N, ctx->saved_data["x"].toIntVector());
         if (ctx->needs_input_grad(1)) dw = product(like, dgu.data_ptr(), ld, 1, o.x, o.ld, o.N, o.K, o.M, {o.N, o.K});
-        return once({dx, dw, Tensor(), Tensor()}, grads);
+        return once({dx, dw, Tensor(), Tensor()}, {{0, 1}, {0, 1}, {}, {}}, grads);
     }
 };
 
@@ -387,4 +405,14 @@ PYBIND11_MODULE(_fastcall, m) {
     m.def("linear", &linear);
     m.def("gated", &gated);
     m.def("q8", &q8);
+    m.def("once", [](const std::vector<OptTensor>& out, const std::vector<Inputs>& inputs, const std::vector<OptTensor>& incoming) {
+        auto defined = [](const std::vector<OptTensor>& v) {
+            std::vector<Tensor> t;
+            for (const OptTensor& o : v) t.push_back(o ? *o : Tensor());
+            return t;
+        };
+        std::vector<OptTensor> back;
+        for (const Tensor& t : once(defined(out), inputs, defined(incoming))) back.push_back(t.defined() ? OptTensor(t) : std::nullopt);
+        return back;
+    });
 }

@@ -15,7 +15,6 @@ import os
 
 import torch
 from torch.autograd.forward_ad import unpack_dual
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -182,9 +181,10 @@ def _product(a, a_ld, a_mn, b, b_ld, b_mn, M, N, K, shape=None) -> torch.Tensor:
     return out
 
 
-def _once(cls, ctx, *gs):
-    """The gradients under torch's guard against a second differentiation (its wrapper costs more than the launches of a small step)."""
-    return once_differentiable(cls.gradients)(ctx, *gs)
+def _once(out, inputs, incoming):
+    """Gradients of a backward pass that records its graph (create_graph): csrc/fastcall.cpp's `once` stands guard over a second differentiation.  `inputs`: for
+    each gradient the positions, among the function's tensor inputs, of those that it depends on."""
+    return (_fast or _bind()).once(out, inputs, incoming)
 
 
 def _scratch(nbytes: int, device) -> torch.Tensor | None:
@@ -230,14 +230,20 @@ class _AddRmsNorm(torch.autograd.Function):
         _norm_forward(x.get_device(), x.shape[-1], x2, r2, wc, eps, y, s, None, None)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x2, r2, wc)
-        ctx.eps, ctx.shape, ctx.rows, ctx.w_dtype = eps, x.shape, x2.shape, wc.dtype if wc is not None else None
+        ctx.eps, ctx.shape, ctx.rows, ctx.w_dtype, ctx.has_residual = eps, x.shape, x2.shape, wc.dtype if wc is not None else None, residual is not None
         return (y, s) if residual is not None else y
 
     @staticmethod
     def backward(ctx, gy, gs=None):
-        if _grad_enabled():  # create_graph: torch marks the gradients as not differentiable again
-            return _once(_AddRmsNorm, ctx, gy, gs)
-        return _AddRmsNorm.gradients(ctx, gy, gs)
+        if not _grad_enabled():
+            return _AddRmsNorm.gradients(ctx, gy, gs)
+        with torch.no_grad():
+            dx, dr, dw, _ = _AddRmsNorm.gradients(ctx, gy, gs)
+        if gy is not None:
+            of_s = [0] + [1] * ctx.has_residual
+            every = of_s + [len(of_s)] * (ctx.w_dtype is not None)
+            dx, dr, dw = _once([dx, dr, dw], [every, every, of_s], [gy, gs])
+        return dx, dr, dw, None
 
     @staticmethod
     def gradients(ctx, gy, gs=None):
@@ -324,13 +330,18 @@ class _LinearAct(torch.autograd.Function):
         _linear_forward(x.get_device(), x.dtype, ops, M, N, K, bias, act, residual, out, z, z_ld)
         ctx.save_for_backward(ops[0], ops[3], z)
         ctx.dims, ctx.saved_shapes, ctx.act, ctx.x_shape = (M, N, K), (ops[0].shape, ops[3].shape), act, x.shape
+        ctx.has_bias = bias is not None
         return out
 
     @staticmethod
     def backward(ctx, gy):
-        if _grad_enabled():
-            return _once(_LinearAct, ctx, gy)
-        return _LinearAct.gradients(ctx, gy)
+        if not _grad_enabled():
+            return _LinearAct.gradients(ctx, gy)
+        with torch.no_grad():
+            dx, dw, db, _, dr = _LinearAct.gradients(ctx, gy)
+        curved = ctx.act > 1  # without an activation, and with relu but for its corner, the slope does not depend on z
+        of_z = [0, 1] + [2] * ctx.has_bias if curved else []
+        return *_once([dx, dw, db], [of_z if curved else [1], of_z if curved else [0], of_z], [gy]), None, dr
 
     @staticmethod
     def gradients(ctx, gy):
@@ -453,9 +464,11 @@ class _GatedLinear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
-        if _grad_enabled():
-            return _once(_GatedLinear, ctx, gy)
-        return _GatedLinear.gradients(ctx, gy)
+        if not _grad_enabled():
+            return _GatedLinear.gradients(ctx, gy)
+        with torch.no_grad():
+            dx, dw, _, _ = _GatedLinear.gradients(ctx, gy)
+        return *_once([dx, dw], [[0, 1], [0, 1]], [gy]), None, None
 
     @staticmethod
     def gradients(ctx, gy):

@@ -124,3 +124,70 @@ def test_forward_mode_is_refused(D, monkeypatch):
         assert not rec.calls
         D.linear_act(bf(2, 64), bf(8, 64))  # without tangents a level changes nothing
         assert len(rec.calls) == 1
+
+
+TWICE = "differentiate twice"
+
+
+def python_calls(D):
+    """Each operator's Python route on leaves; the values are whatever the memory holds, the graph is what is looked at."""
+    leaf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, requires_grad=True)  # noqa: E731
+    x, w, b, r = leaf(4, 64), leaf(16, 64), leaf(16), leaf(4, 16)
+    n, s = leaf(64), leaf(4, 64)
+    w13 = leaf(32, 64)
+    return [("linear", (x, w, b, r), lambda: D._LinearAct.apply(x, w, b, 3, r)), ("gated", (x, w13), lambda: D._GatedLinear.apply(x, w13, 2, 0.0)), ("norm", (x, s, n), lambda: D._AddRmsNorm.apply(x, s, n, 1e-6)[0])]
+
+
+def check_guard(calls):
+    for name, leaves, f in calls:
+        for gy_wants in (False, True):
+            y = f()
+            gy = torch.ones_like(y).requires_grad_(gy_wants)
+            gs = torch.autograd.grad(y, leaves, gy, create_graph=True)
+            for i, g in enumerate(gs[:2]):  # x and w (or the norm's residual) depend on all the others
+                loss = y.float().sum() + g.float().square().sum()
+                for leaf in leaves[:2] + ((gy,) if gy_wants else ()):
+                    with pytest.raises(RuntimeError, match=TWICE):
+                        torch.autograd.grad(loss, leaf, retain_graph=True)
+                with pytest.raises(RuntimeError, match=TWICE):
+                    loss.backward(retain_graph=True)
+            plain = torch.autograd.grad(y, leaves, gy.detach(), retain_graph=True)
+            assert not any(g.requires_grad for g in plain)
+
+
+def test_second_derivatives_raise_on_the_way_to_any_input(D, monkeypatch):
+    Recorder(D, monkeypatch)
+    check_guard(python_calls(D))
+
+
+def check_free(linear, dtype=torch.bfloat16, device="cpu"):
+    """Gradients that depend on nothing that wants one stay as they are; the residual's is the incoming one and can be differentiated again; without an activation
+    the gradient of x depends on w alone and that of w on x alone."""
+    t = lambda *s: torch.ones(*s, dtype=dtype, device=device)  # noqa: E731
+    for act in (None, "relu"):
+        x = t(4, 64).requires_grad_(True)
+        y = linear(x, t(16, 64), t(16), act, t(4, 16))
+        assert not torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)[0].requires_grad
+        b = t(16).requires_grad_(True)
+        y = linear(t(4, 64), t(16, 64), b, act, None)
+        assert not torch.autograd.grad(y, b, torch.ones_like(y), create_graph=True)[0].requires_grad
+    r, x = t(4, 16).requires_grad_(True), t(4, 64).requires_grad_(True)
+    y = linear(x, t(16, 64), None, "silu", r)
+    v = t(4, 16).requires_grad_(True)
+    dr = torch.autograd.grad(y, r, v, create_graph=True)[0]
+    assert torch.equal(torch.autograd.grad((dr * dr).sum(), v)[0], 2 * v.detach())
+    for act in (None, "relu"):
+        x, w, b = t(4, 64).requires_grad_(True), t(16, 64).requires_grad_(True), t(16).requires_grad_(True)
+        y = linear(x, w, b, act, None)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y), create_graph=True)
+        assert dx.requires_grad and dw.requires_grad and not db.requires_grad
+        for g, free, bound in ((dx, x, w), (dw, w, x)):
+            assert torch.autograd.grad(g.float().sum(), (free, b), allow_unused=True, retain_graph=True) == (None, None)
+            torch.autograd.grad(y.float().sum() + g.float().sum(), (free, b), retain_graph=True)
+            with pytest.raises(RuntimeError, match=TWICE):
+                torch.autograd.grad(y.float().sum() + g.float().sum(), bound, retain_graph=True)
+
+
+def test_gradients_that_depend_on_nothing_are_free(D, monkeypatch):
+    Recorder(D, monkeypatch)
+    check_free(lambda x, w, b, act, r: D._LinearAct.apply(x, w, b, D._act_code(act), r))

@@ -4,6 +4,8 @@ import importlib
 import pytest
 import torch
 
+from test_dense_autograd_host import check_free, check_guard
+
 pytestmark = pytest.mark.gpu
 T = torch.bfloat16
 
@@ -108,3 +110,24 @@ def test_forward_mode_is_refused(D, dev, kind):
     x, w = randn((4, 64), 1, dev), randn((8, 64), 2, dev)
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.func.jvp(lambda a: D.linear_act(a, w), (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("kind", ["dense", "slices", "odd"])  # dense: the extension's functions; slices and odd offsets: dense.py's
+def test_second_derivatives_raise_on_the_way_to_any_input(D, dev, kind):
+    """Constant and differentiable incoming gradients, whichever leaf is asked for; and a penalty on a gradient does not train without its own gradient."""
+    check_guard([(name, tuple(leaves), f) for name, leaves, f in calls(D, dev, kind) if name != "product"])
+    for name, leaves, f in calls(D, dev, kind):
+        y = f()
+        gy = randn(y.shape, 9, dev)
+        plain = torch.autograd.grad(y, leaves, gy, retain_graph=True)
+        graph = torch.autograd.grad(y, leaves, gy, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+
+
+@pytest.mark.parametrize("odd", [False, True])
+def test_gradients_that_depend_on_nothing_are_free(D, dev, odd):
+    def linear(x, w, b, act, r):
+        if odd:  # rows that are no view of 16-byte ones: dense.py's functions
+            x = torch.cat([x, x], 1)[:, 3:67]
+        return D.linear_act(x, w, b, act, r)
+    check_free(linear, T, dev)
