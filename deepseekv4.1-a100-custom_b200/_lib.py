@@ -103,6 +103,7 @@ _SIGNATURES = {
     "b200_gated_linear": (c_i, [c_p, c_ll, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_f, c_p, c_ll, c_p, c_ll, c_p]),
     "b200_gated_linear_bwd": (c_i, [c_p, c_ll, c_p, c_ll, c_i, c_f, c_i, c_i, c_i, c_p, c_ll, c_p]),
     "b200_dense_product": (c_i, [c_p, c_ll, c_i, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p, c_ll, c_p]),
+    "b200_dense_tile": (c_i, [c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_p]),
     "b200_align_rows": (c_i, [c_p, c_ll, c_p, c_ll, c_p, c_ll, c_p, c_ll, c_i, c_ll, c_p]),
     "b200_linear_act_q8_workspace_bytes": (c_sz, [c_i, c_i, c_i]),
     "b200_linear_act_q8": (c_i, [c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_ll, c_p, c_ll, c_p, c_sz, c_p]),

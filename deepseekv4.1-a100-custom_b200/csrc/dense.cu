@@ -193,6 +193,21 @@ extern "C" int b200_dense_product(const void* a_base, long long a_ld, int a_mn, 
     return fg_launch(a, stream);
 }
 
+extern "C" int b200_dense_tile(int M, int N, int K, int gated, int a_mn, int b_mn, int fp8, int has_residual, int single_values, int sms, int* tile) {
+    if (M <= 0 || N <= 0 || K <= 0 || sms < 4 || !tile) return ERR_BAD_ARG;
+    if (too_large(M, N, K)) return ERR_TOO_LARGE;
+    FgArgs a{};
+    a.a.mn_major = a_mn != 0;
+    a.b.mn_major = b_mn != 0;
+    a.M = M; a.N = N; a.K = fp8 ? K / 2 : K;
+    a.dual = gated != 0;
+    a.inter = N / 2;
+    if (fp8) a.xsf = reinterpret_cast<const uint8_t*>(tile);  // what follows looks only at whether there are scales and a residual
+    if (has_residual) a.res = tile;
+    fg_tile(a, single_values, sms, tile);
+    return 0;
+}
+
 extern "C" size_t b200_linear_act_bwd_workspace_bytes(int M, int N) {
     if (M <= 0 || N <= 0) return 0;
     return (size_t)((M + DZ_ROWS - 1) / DZ_ROWS) * (size_t)N * sizeof(float);

@@ -747,12 +747,12 @@ static int fg_layouts(FgParams& P, cudaStream_t stream) {
 // 8192 x 8192 x 8192; e.g. measured 64 x 4096 x 4096: 1/128/4 13.9, 1/128/1 20.9, 2/256/1 25.7; 512 x 4096 x 4096: 2/256/2 21.3, 1/128/1 22.0,
 // 1/128/4 47.5; 1500 x 4096 x 4096: 2/192/1 41.9, 2/256/1 48.0, 1/128/1 55.9; 4096 x 12288 x 4096: 2/256/1 275, 2/192/1 290, 1/128/1 384.
 // FP8: 64 x 4096 x 4096: 1/128/4 14.4, 1/128/1 19.5, 2/192/1 24.1; 4096 x 12288 x 4096: 2/192/1 202, 1/128/1 249.
-static FgPick fg_pick(const FgParams& P) {
+static FgPick fg_pick(const FgParams& P, int sms) {
     const FgArgs& g = P.g;
     static const struct { FgPick k; double stage, stage_mx, fixed, epi, epi_res; } choices[] = {
-        {{1, 128, 1}, .54, .76, 4.0, 2.5, 4.8}, {{1, 128, 2}, .54, .69, 7.5, 0, 0},      {{1, 128, 4}, .54, .69, 8.5, 0, 0},      {{2, 128, 1}, .54, .76, 4.5, 2.8, 5.0},
-        {{2, 128, 2}, .54, .70, 8.0, 0, 0},     {{2, 192, 1}, .645, .83, 5.5, 4.2, 7.5}, {{2, 256, 1}, .78, 0, 6.5, 5.0, 9.0}, {{2, 256, 2}, .78, 0, 10.0, 0, 0}};
-    const int st = (g.K + 2 * FG_BK - 1) / (2 * FG_BK), sms = sm_count();
+        {{1, 128, 1}, .54, .76, 4.0, 2.5, 4.8},  {{1, 128, 2}, .54, .69, 7.5, 0, 0},    {{1, 128, 4}, .54, .69, 8.5, 0, 0},
+        {{2, 192, 1}, .645, .83, 5.5, 4.2, 7.5}, {{2, 256, 1}, .78, 0, 6.5, 5.0, 9.0}, {{2, 256, 2}, .78, 0, 10.0, 0, 0}};
+    const int st = (g.K + 2 * FG_BK - 1) / (2 * FG_BK);
     FgPick best{1, 128, 1};
     double best_t = 1e30;
     for (const auto& c : choices) {
@@ -771,12 +771,22 @@ static FgPick fg_pick(const FgParams& P) {
 
 template <typename T>
 static int fg_dispatch(FgParams& P, cudaStream_t stream) {
-    const FgPick k = fg_pick(P);
+    const FgPick k = fg_pick(P, sm_count());
     P.split = k.split;
     if (k.cg == 1) return k.split > 1 ? fg_layouts<T, 1, 128, true>(P, stream) : fg_layouts<T, 1, 128, false>(P, stream);
-    if (k.bn == 128) return k.split > 1 ? fg_layouts<T, 2, 128, true>(P, stream) : fg_layouts<T, 2, 128, false>(P, stream);
     if (k.bn == 192) return fg_layouts<T, 2, 192, false>(P, stream);
     return k.split > 1 ? fg_layouts<T, 2, 256, true>(P, stream) : fg_layouts<T, 2, 256, false>(P, stream);
+}
+
+// the products of up to FS_MAX_M rows with K-major 16-bit operands are fstream.cu's
+static bool fg_streams(const FgArgs& a) { return a.M <= FS_MAX_M && !a.a.mn_major && !a.b.mn_major && !a.xsf; }
+
+void fg_tile(const FgArgs& a, int single_values, int sms, int* tile) {
+    FgParams P{};
+    P.g = a;
+    P.turned = !a.xsf && single_values;
+    const FgPick k = a.M <= FS_MAX_M && (a.xsf || fg_streams(a)) ? FgPick{0, 0, 0} : fg_pick(P, sms);
+    tile[0] = k.cg; tile[1] = k.bn; tile[2] = k.split;
 }
 
 int fg_launch(const FgArgs& a, cudaStream_t stream) {
@@ -785,7 +795,7 @@ int fg_launch(const FgArgs& a, cudaStream_t stream) {
     if (a.dual && (a.N != 2 * a.inter || a.b.mn_major)) return ERR_BAD_SHAPE;
     if (((uintptr_t)a.a.base & 15) || ((uintptr_t)a.b.base & 15) || a.a.ld % 8 || a.b.ld % 8) return ERR_BAD_ALIGN;
     if (a.a.ld < (a.a.mn_major ? a.M : a.K) || a.b.ld < (a.b.mn_major ? a.N : a.K)) return ERR_BAD_SHAPE;
-    if (a.M <= FS_MAX_M && !a.a.mn_major && !a.b.mn_major && !a.xsf) return fs_launch(a, stream);
+    if (fg_streams(a)) return fs_launch(a, stream);
     FgParams P{};
     P.g = a;
     auto vec = [](const void* p, long long ld_bytes) {

@@ -42,6 +42,9 @@ struct FgArgs {
 size_t fg_sf_workspace_bytes(int M, int N, int K_pairs);
 
 int fg_launch(const FgArgs& a, cudaStream_t stream);
+// the kernel that a call would take on `sms` SMs: {CTAs of a tile, its columns, ways k is split}, zeros for the weight-streaming kernel; single_values: a row of the
+// result, the residual or z does not start on 16 bytes
+void fg_tile(const FgArgs& a, int single_values, int sms, int* tile);
 // fstream.cu: the same for M <= FS_MAX_M, K-major operands
 constexpr int FS_MAX_M = 16;
 int fs_launch(const FgArgs& a, cudaStream_t stream);

@@ -535,9 +535,9 @@ static int norm_bwd_per_sm(int dim) {
     return n > 16 ? 16 : n;
 }
 
-template <typename T, int NV>
+template <typename T>
 static int bwd_ring(const NormArgs& a, int tpr, int stages, size_t smem, int grid, cudaStream_t stream) {
-    auto kernel = add_rms_norm_bwd_ring_kernel<T, NV>;
+    auto kernel = add_rms_norm_bwd_ring_kernel<T, 2>;
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -552,13 +552,13 @@ static int bwd_ring(const NormArgs& a, int tpr, int stages, size_t smem, int gri
 template <typename T>
 static int bwd_typed(const NormArgs& a, bool vec, int grid, cudaStream_t stream) {
     const BwdShape b = norm_bwd_shape(a.dim, vec);
-    if (vec && b.nv <= 2) {
+    if (vec && b.nv == 2) {
         const size_t stage = (size_t)(2 + (a.r != nullptr) + (a.gs != nullptr)) * a.dim * sizeof(T);
         int stages = (int)(NORM_RING_BYTES / norm_bwd_per_sm(a.dim) / stage);
         if (stages > NORM_MAX_STAGES) stages = NORM_MAX_STAGES;
-        if (stages >= 3) return b.nv == 1 ? bwd_ring<T, 1>(a, b.tpr, stages, stages * stage, grid, stream) : bwd_ring<T, 2>(a, b.tpr, stages, stages * stage, grid, stream);
+        if (stages >= 3) return bwd_ring<T>(a, b.tpr, stages, stages * stage, grid, stream);
     }
-    void (*k)(const NormArgs, int) = vec ? (b.nv == 1 ? add_rms_norm_bwd_kernel<T, 8, 1> : b.nv == 2 ? add_rms_norm_bwd_kernel<T, 8, 2> : add_rms_norm_bwd_kernel<T, 8, 4>)
+    void (*k)(const NormArgs, int) = vec ? (b.nv == 2 ? add_rms_norm_bwd_kernel<T, 8, 2> : add_rms_norm_bwd_kernel<T, 8, 4>)
                                          : (b.nv == 4 ? add_rms_norm_bwd_kernel<T, 1, 4> : add_rms_norm_bwd_kernel<T, 1, 16>);
     return (int)launch_pdl(k, dim3(grid), dim3(b.tpr), 0, stream, a, b.tpr);
 }

@@ -392,6 +392,9 @@ int b200_dense_product(const void* a, long long a_ld, int a_mn, const void* b, l
                        cudaStream_t stream);
 int b200_align_rows(const void* src, long long src_ld, void* dst, long long rows, const void* src2, long long src2_ld, void* dst2, long long rows2, int cols,
                     long long dst_ld, cudaStream_t stream);
+/* the kernel that such a product of N columns (gated: gate and up together) takes on a GPU of `sms` SMs: tile[0..2] = CTAs that share a tile, its columns,
+ * ways its k is split; zeros: the weight-streaming kernel of few rows.  single_values: a row of the result, residual or z does not start on 16 bytes. */
+int b200_dense_tile(int M, int N, int K, int gated, int a_mn, int b_mn, int fp8, int has_residual, int single_values, int sms, int* tile);
 size_t b200_linear_act_q8_workspace_bytes(int M, int N, int K);
 int b200_linear_act_q8(const void* x8, const void* xsf, const void* w8, const void* s8, int s_cols, int M, int N, int K, const void* bias, int act, const void* residual,
                        long long r_ld, void* out, long long out_ld, void* workspace, size_t workspace_bytes, cudaStream_t stream);
