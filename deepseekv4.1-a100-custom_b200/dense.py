@@ -527,6 +527,7 @@ class DenseFFN:
         self.inter, self.dim = w13.shape[0] // 2, w13.shape[1]
         assert tuple(w2.shape) == (self.dim, self.inter) and w13.shape[0] == 2 * self.inter, f"w13 {tuple(w13.shape)} does not fit w2 {tuple(w2.shape)}"
         _act_code(act)
+        assert limit >= 0.0, "limit must not be negative"
         self._nat = None
         if isinstance(w13, W8) or isinstance(w2, W8):
             assert isinstance(w13, W8) and isinstance(w2, W8) and w13.s8.dtype == torch.uint8 and w2.s8.dtype == torch.uint8, "w13 and w2: two W8 with E8M0 scales"
