@@ -18,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 LIB = os.path.join(HERE, "libb200moe.so")
 FASTCALL = os.path.join(HERE, "_fastcall.so")
+FASTCALL_KEY = os.path.join(HERE, "_obj", "fastcall.key")
 NVCC = os.environ.get("B200MOE_NVCC", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -52,21 +53,39 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def fastcall_key() -> str:
+    """What _fastcall.so is built against: it links torch's C++ interface, which another torch or Python does not share."""
+    import torch
+    return f"torch {torch.__version__}, python {sys.version.split()[0]}, cxx11 abi {int(torch.compiled_with_cxx11_abi())}\n"
+
+
+def fastcall_up_to_date() -> bool:
+    src = os.path.join(HERE, "fastcall.cpp")
+    if not os.path.exists(FASTCALL) or not os.path.exists(FASTCALL_KEY):
+        return False
+    with open(FASTCALL_KEY) as f:
+        return f.read() == fastcall_key() and all(os.path.getmtime(d) <= os.path.getmtime(FASTCALL) for d in (src, os.path.abspath(__file__)))
+
+
 def build_fastcall(force: bool = False) -> str:
     """fastcall.cpp against the installed torch (host code only)."""
-    src = os.path.join(HERE, "fastcall.cpp")
-    if not force and os.path.exists(FASTCALL) and all(os.path.getmtime(d) <= os.path.getmtime(FASTCALL) for d in (src, os.path.abspath(__file__))):
+    if not force and fastcall_up_to_date():
         return FASTCALL
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension as ext
     inc = [*ext.include_paths(), sysconfig.get_paths()["include"], os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")]
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f for i in inc for f in ("-isystem", i)), src,
-           "-o", FASTCALL, *(f"-L{d}" for d in ext.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f for i in inc for f in ("-isystem", i)),
+           os.path.join(HERE, "fastcall.cpp"), "-o", FASTCALL, *(f"-L{d}" for d in ext.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if os.path.exists(FASTCALL_KEY):
+        os.remove(FASTCALL_KEY)  # a build that is cut short leaves no key
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"g++ failed for fastcall.cpp:\n{r.stdout}\n{r.stderr}")
+    os.makedirs(os.path.dirname(FASTCALL_KEY), exist_ok=True)
+    with open(FASTCALL_KEY, "w") as f:
+        f.write(fastcall_key())
     return FASTCALL
 
 
