@@ -75,8 +75,10 @@ enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TA
 __device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
 // Phi(z), the normal distribution function: erfc by the rational approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
-// Functions (|error| <= 1.5e-7), taken on the side where it is small, so that Phi of a negative z does not come out of a cancellation.
-// A third of the instructions of 0.5 (1 + erff(..)), which made the epilogue of a large tile longer than the products under it.
+// Functions, taken on the side where it is small, so that Phi of a negative z does not come out of a cancellation.  |error| of Phi <= 0.75e-7.  Its relative
+// error grows down the tail: 5e-5 at z = -3, 5e-4 at -4, 1.6e-3 at -5, 1 % at -8 (0.5 (1 + erff(..)) in fp32: 8e-4 at -4, 8 % at -5, nothing left at -6).
+// z Phi(z) is therefore off by half a step of fp16 more around z = -4, where it is -1.3e-4, and by more than half a step of bf16 below z = -5.5, where it
+// is smaller than 1.1e-7.  A third of the instructions of 0.5 (1 + erff(..)), which made the epilogue of a large tile longer than the products under it.
 __device__ __forceinline__ float normal_cdf(float z) {
     const float a = fabsf(z) * 0.70710678118654752f, t = __fdividef(1.f, 1.f + 0.3275911f * a);
     const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));

@@ -231,3 +231,17 @@ def test_sums_fit_fp32():
     assert longest < 2 ** 24 and max(max(s) for t in (shapes.BACKWARD, shapes.BACKWARD_ODD) for s in t) < 2 ** 24
     assert (9 * 0.67 * math.sqrt(5600)) ** 2 < 2 ** 24
     assert max(k for _, _, k in shapes.FP8) * 2 ** 4 * 2 ** 4 < 2 ** 24
+
+
+@both
+@pytest.mark.parametrize("m", [8, 400])
+def test_gelu_tail(D, dev, dt, m):
+    """gelu of -12 .. 4 through an identity weight: Phi is off by 0.75e-7 at most and by 5 % at most below -8, and z Phi(z) is rounded once."""
+    t = TYPES[dt]
+    z = torch.linspace(-12, 4, m * 8, device=dev).to(t).view(m, 8)
+    y = D.linear_act(z, torch.eye(8, device=dev, dtype=t), None, "gelu").double()
+    z = z.double()
+    ref = z * 0.5 * torch.erfc(-z / math.sqrt(2))  # 1 + erf would cancel, in 64 bits too: off by 1e-16, more than the values from z = -8.3 on
+    e = z.abs() * 0.75e-7 + 2.0 ** -20 * ref.abs()
+    e = torch.where(z < -8, torch.minimum(e, 0.05 * ref.abs()), e)
+    within(y, ref, u_of(t) * (ref.abs() + e) + e + tiny_of(t), "gelu")
