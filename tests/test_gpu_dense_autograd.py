@@ -131,3 +131,16 @@ def test_gradients_that_depend_on_nothing_are_free(D, dev, odd):
             x = torch.cat([x, x], 1)[:, 3:67]
         return D.linear_act(x, w, b, act, r)
     check_free(linear, T, dev)
+
+
+@pytest.mark.parametrize("kind", ["dense", "slices", "odd"])
+def test_checkpointed_calls(D, dev, kind):
+    """torch.utils.checkpoint hands the tensors of a second forward pass to the backward pass: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    for name, leaves, f in calls(D, dev, kind):
+        y = f()
+        gy = randn(y.shape, 9, dev)
+        ref = torch.autograd.grad(y, leaves, gy)
+        y2 = checkpoint(f, use_reentrant=False)
+        got = torch.autograd.grad(y2, leaves, gy)
+        assert torch.equal(y, y2) and all(torch.equal(a, b) for a, b in zip(got, ref)), name
