@@ -405,6 +405,11 @@ PYBIND11_MODULE(_fastcall, m) {
     m.def("linear", &linear);
     m.def("gated", &gated);
     m.def("q8", &q8);
+    m.def("tangents", [](const std::vector<OptTensor>& ts) {
+        for (const OptTensor& t : ts)
+            if (dual(t)) return true;
+        return false;
+    });
     m.def("once", [](const std::vector<OptTensor>& out, const std::vector<Inputs>& inputs, const std::vector<OptTensor>& incoming) {
         auto defined = [](const std::vector<OptTensor>& v) {
             std::vector<Tensor> t;

@@ -14,7 +14,6 @@ import importlib.util
 import os
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib as L
 
@@ -171,7 +170,7 @@ def _wants_grad(a, b=None, c=None, d=None) -> bool:
 
 def _no_tangents(*ts) -> None:
     """Inputs that carry a forward-mode tangent are refused: the result would have none, which torch takes for a derivative of zero."""
-    if any(t is not None and unpack_dual(t).tangent is not None for t in ts):
+    if (_fast or _bind()).tangents(ts):
         raise NotImplementedError("the dense operators have no forward-mode derivatives")
 
 
