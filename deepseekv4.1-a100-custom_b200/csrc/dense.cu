@@ -9,7 +9,8 @@
 namespace b200 {
 
 // dz = gy * act'(z) and the column sums of dz.  z arrives in fp32: in 16 bits its rounding would put an error of the size of the result's own
-// rounding into every gradient.  8 warps of a block share DZ_ROWS rows of 32 * VEC columns; the sums of a block's rows go to
+// rounding into every gradient.  dz leaves in T, since the tensor cores multiply 16-bit values (as torch's 16-bit linear does): the gradients' error against
+// 64 bits is 0.00029 in place of 0.00021 of an fp32 dz in fp16, 0.0023 in place of 0.0017 in bf16.  8 warps of a block share DZ_ROWS rows of 32 * VEC columns; the sums of a block's rows go to
 // part[row block][N] in fp32 (from the unrounded dz), added in block order afterwards.  Row and column blocks share grid x (y ends at 65535, which would
 // end the rows at 4.2 million).  Bound by HBM: gy and z in, dz out.
 constexpr int DZ_ROWS = 64;
@@ -56,7 +57,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, 
 }
 
 // [dg | du] of the gated product from gy and the saved [g | u]: dg = gy u' act'(g') where the clamp let g through, du = gy act(g') where it
-// let u through (g', u': the clamped values).  g and u arrive in fp32 (as z above).  Bound by HBM: 10 bytes in, 4 out per element of gy.
+// let u through (g', u': the clamped values).  g and u arrive in fp32, dg and du leave in T (as z and dz above).  Bound by HBM: 10 bytes in, 4 out per element of gy.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) gated_bwd_kernel(const T* __restrict__ gy, long long gy_ld, const float* __restrict__ gu, long long gu_ld, int act, float limit, long long M,
                                                         int inter, T* __restrict__ dgu, long long dgu_ld) {

@@ -1,6 +1,6 @@
-// Short way from Python to the calls of the dense operators.  A one-token call is bound by the host: through ctypes and torch's Python it takes 10 to
-// 14 us, of which the launch is 3; from here 4 to 6.  A training step of one small projection takes 132 us with autograd functions in Python and 76
-// with the ones here (torch's own linear: 98).  Each function takes the plain case only (CUDA tensors of one device, the current one; contiguous;
+// Short way from Python to the calls of the dense operators.  A one-token call is bound by the host: through ctypes and torch's Python it takes 13 us, of
+// which the launch is 3; from here 4.4 (a projection) to 6.4 (a norm in 8 bits with its three outputs), calls in a row.  A training step of one
+// 32 x 64 x 64 projection with silu takes 125 us with autograd functions in Python and 68 with the ones here (torch's own linear: 83, with silu 104).  Each function takes the plain case only (CUDA tensors of one device, the current one; contiguous;
 // shapes and types that fit) and answers None to everything else, which dense.py then checks, refuses or lays out.  The kernels are the same
 // entry points of libb200moe.so; their addresses are handed in once by dense.py.
 #include <ATen/ATen.h>

@@ -7,7 +7,7 @@
 //   warp 0      TMA producer: 64-deep k blocks of both operands into a ring of shared-memory stages (128-byte swizzle)
 //   warp 1      one thread (of the first CTA of a pair) issues the MMAs; the accumulators live in TMEM, two buffers, so that the epilogue of
 //               a tile runs under the MMAs of the next
-//   warps 4-11  epilogue: a thread owns one output row (TMEM lane) and half of the tile's columns
+//   warps 4-11  epilogue: a thread owns one output row (TMEM lane) and half of the tile's columns (168 registers; 60 to 68 bytes spill)
 // Every wait is bounded; one that runs out of time records a code in a device error word and the CTA runs to its end.
 #include "fgemm.cuh"
 
@@ -745,8 +745,11 @@ static int fg_layouts(FgParams& P, cudaStream_t stream) {
 // Which tile, and how many ways its k is split.  Each choice's time is estimated as (turns of the busiest CTA) x (time of a tile: its stages' products, or
 // its epilogue where that is longer) + (start, end and last epilogue), the constants in us from measurements over 25 shapes between 64 x 4096 x 2048 and
 // 8192 x 8192 x 8192; e.g. measured 64 x 4096 x 4096: 1/128/4 13.9, 1/128/1 20.9, 2/256/1 25.7; 512 x 4096 x 4096: 2/256/2 21.3, 1/128/1 22.0,
-// 1/128/4 47.5; 1500 x 4096 x 4096: 2/192/1 41.9, 2/256/1 48.0, 1/128/1 55.9; 4096 x 12288 x 4096: 2/256/1 275, 2/192/1 290, 1/128/1 384.
-// FP8: 64 x 4096 x 4096: 1/128/4 14.4, 1/128/1 19.5, 2/192/1 24.1; 4096 x 12288 x 4096: 2/192/1 202, 1/128/1 249.
+// 1/128/4 47.5; 1500 x 4096 x 4096: 2/192/1 41.9, 2/256/1 48.0, 1/128/1 55.9; 4096 x 12288 x 4096: 2/256/1 275, 2/192/1 290, 1/128/1 384 (single products on a
+// cool device; the last one takes 303 in a loop with gelu and 351 among other work, under the 1000 W limit).
+// FP8: 64 x 4096 x 4096: 1/128/4 14.4, 1/128/1 19.5, 2/192/1 24.1; 4096 x 12288 x 4096: 2/192/1 202, 1/128/1 249; 4096 x 4096 x 2048: 2/192/1 47 and with a
+// residual 55, where the estimate is 39 and 43.
+// 128-column tiles of a pair are not compiled: they cost what 128 x 128 tiles of one SM cost or more, in as many turns or more.
 static FgPick fg_pick(const FgParams& P, int sms) {
     const FgArgs& g = P.g;
     static const struct { FgPick k; double stage, stage_mx, fixed, epi, epi_res; } choices[] = {
@@ -806,6 +809,7 @@ int fg_launch(const FgArgs& a, cudaStream_t stream) {
     P.vec_res = vec(a.res, a.res_ld * 2);
     P.vec_z = vec(a.z_out, a.dual ? a.z_ld * 4 | a.inter * 4 : a.z_ld * 4);
     P.vec_bias = vec(a.bias, 0);
+    // FP8 has no room for the turning buffer: its single values are stored 32 rows apart (4096 x 4097 x 2048 with residual 197 us, 4096 x 4096 x 2048 55)
     P.turned = !a.xsf && (!P.vec_out || (a.res && !P.vec_res) || (a.z_out && !P.vec_z));
     return a.is_f16 ? fg_dispatch<__half>(P, stream) : fg_dispatch<__nv_bfloat16>(P, stream);
 }

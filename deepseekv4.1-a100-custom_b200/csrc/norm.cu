@@ -5,10 +5,14 @@
 // norm itself uses the unrounded fp32 sum, and the backward pass adds x and r again instead of reading the rounded s, so that the only
 // roundings are those of the outputs.
 //
-// All three are bound by HBM: a row is read once, held in registers as fp32 and written once (forward 4 arrays, 8-bit form 3.5, backward 5).
+// All three are bound by HBM: a row is read once, held in registers (wide rows and most backward passes: in shared memory) and written once (forward 4
+// arrays, 8-bit form 3.5, backward 5).
 // A row belongs to tpr threads, each with NV vectors of 8 values (or single values where the width or an address does not allow 16-byte
-// accesses); one reduction per row.  Measured (bf16, graph replay): one row of 4096 2.2 us; 8191 x 4096 46.2 us (5.8 TB/s); 4099 x 5120 in 8 bits
-// 27.9 us (5.3 TB/s); backward 8191 x 4096 60.9 us (5.5 TB/s), the column sum of dw included.
+// accesses); one reduction per row.  Measured (graph replay): bf16 one row of 4096 2.0 us; 8191 x 4096 46.5 us (5.8 TB/s); 4099 x 5120 in 8 bits
+// 27.9 us (5.3 TB/s); 4099 x 16384 104 us (5.2 TB/s); fp32 8191 x 4096 83.5 us (6.4 TB/s); backward, the column sum of dw included, 8191 x 4096 61.9 us in
+// bf16 (5.4 TB/s) and 131 in fp32 (5.1 TB/s).  Far from that: the backward pass of widths above 8192 (2048 x 16384 204 us in bf16, 1.6 TB/s) and of widths
+// that are no multiple of 8 (8191 x 4095 252 us, 8191 x 4097 1535 us), whose register kernels spill 0.9 to 2.7 KB per thread above 8192 and, in single
+// values, above 4096.
 #include <cuda_fp8.h>
 
 #include "b200_moe.h"

@@ -4,9 +4,9 @@ bias, activation and residual in its epilogue (`linear_act`, `linear_act_q8`), t
 tensors' device; nothing synchronises.  Scratch and outputs come from torch's allocator per call, so calls on several streams, and captured
 CUDA graphs, share no memory.
 
-`add_rms_norm`, `linear_act` and `gated_linear` are differentiable (once, in reverse mode; inputs with a forward-mode tangent are
-refused); the FP8 forms are for serving and refuse inputs that require a gradient.  A captured backward pass needs what torch asks of any: capture it on the stream that ran the warm-up, and drop eager graphs of the
-same leaves first."""
+`add_rms_norm`, `linear_act` and `gated_linear` are differentiable in reverse mode, once: gradients of a create_graph backward raise when they are
+differentiated again, and inputs with a forward-mode tangent are refused.  The FP8 forms are for serving and refuse inputs that require a gradient.
+A captured backward pass needs what torch asks of any: capture it on the stream that ran the warm-up, and drop eager graphs of the same leaves first."""
 from __future__ import annotations
 
 import ctypes
@@ -23,7 +23,7 @@ _ACT = L.ACTIVATIONS
 # ------------------------------------------------------------------ marshalling
 # The small calls of a decode step are bound by the host, so nothing here builds objects that a call does not need: addresses go to ctypes as
 # plain integers, the stream is read without a Stream object, contiguous tensors without a view, and the device is switched only when it is not
-# the current one (one-row norm 20 -> 12 us, one-row projection 20 -> 10 us; plain calls do not come here, they take csrc/fastcall.cpp's 5 and 4 us).
+# the current one (a norm or a projection of few strided rows: 13 us, calls in a row; plain calls do not come here, they take csrc/fastcall.cpp's 4.4 to 6.4).
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _functions: dict = {}
@@ -516,8 +516,9 @@ class DenseFFN:
     behind the block.
 
     w13 [2 * inter, D] and w2 [D, inter]: bf16 or fp16 tensors (trainable: every step is differentiable), or `W8` containers with E8M0 scales (D and
-    inter multiples of 128, serving only): the normed rows and the gated product then stay in 8 bits between the steps.  A natural-k-order copy of
-    the W8 bytes is made once here, as MoELayer does for the shared expert."""
+    inter multiples of 128, serving only): the normed rows and the gated product then stay in 8 bits between the steps, and with a limit the
+    clamps take a NaN for the limit, as the expert kernels' do (in 16 bits it stays one).  A natural-k-order copy of the W8 bytes is made once here, as MoELayer
+    does for the shared expert."""
 
     def __init__(self, norm_weight: torch.Tensor | None, w13, w2, *, eps: float = 1e-6, act: str = "silu", limit: float = 0.0):
         from .w8 import W8, unpermute_k
